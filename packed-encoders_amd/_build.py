@@ -35,7 +35,7 @@ HIPCC_FLAGS = [
     "-mllvm", "-amdgpu-mfma-vgpr-form",
 ]
 EXTENSION = HERE / "_pe_torch.so"  # native launches for torch tensors (csrc/pe_torch.cpp)
-SOURCES = ["pe_attn_capi.hip"]
+SOURCES = ["pe_attn_capi.hip", "pe_paged.hip"]
 PEAKS_SOURCES = ["pe_peaks.hip"]
 
 
@@ -49,10 +49,12 @@ def _code_only(text: str) -> str:
 
 def source_digest() -> str:
     """A short sha256 over the code of the attention library's HIP sources and public header
-    (comments and layout excluded; the peaks microbenchmarks are not part of it) and the
-    compile flags: what ties a committed profile of the kernels to the code it measured."""
+    (comments and layout excluded; the peaks microbenchmarks and the paged cache, which no
+    profiled workload runs, are not part of it) and the compile flags: what ties a committed
+    profile of the kernels to the code it measured."""
     h = hashlib.sha256(" ".join(HIPCC_FLAGS).encode())
-    files = [p for p in [*CSRC.iterdir(), *INCLUDE.iterdir()] if p.is_file() and "peaks" not in p.name]
+    files = [p for p in [*CSRC.iterdir(), *INCLUDE.iterdir()]
+             if p.is_file() and "peaks" not in p.name and "pe_paged" not in p.name]
     for path in sorted(files):
         h.update(path.name.encode())
         h.update(_code_only(path.read_text()).encode())

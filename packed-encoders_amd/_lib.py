@@ -39,6 +39,17 @@ EXPORTED = (
     "pe_layer_norm_fwd",
     "pe_geglu_fwd",
 )
+# include/pe_paged.h
+PAGED_EXPORTED = (
+    "pe_paged_workspace_size",
+    "pe_paged_attn_fwd",
+    "pe_rotary_fwd",
+    "pe_paged_append_fwd",
+    "pe_copy_pages",
+)
+PAGE_MULTIPLE = 16      # PE_PAGED_PAGE_MULTIPLE
+ROTARY_MAX_PAIRS = 256  # PE_ROTARY_MAX_PAIRS
+ROTARY_BF16, ROTARY_FP16, ROTARY_FP32 = 1, 2, 3
 
 
 class AttnArgs(ctypes.Structure):
@@ -107,6 +118,55 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class PagedArgs(ctypes.Structure):
+    """Mirror of ``pe_paged_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        *[(name, ctypes.c_void_p) for name in ("q", "k_pages", "v_pages", "o", "page_table", "cu_seqlens", "seqlens_k")],
+        *[(name, ctypes.c_int64) for name in (
+            "q_stride_token", "q_stride_head", "k_stride_page", "k_stride_token", "k_stride_head", "v_stride_page",
+            "v_stride_token", "v_stride_head", "o_stride_token", "o_stride_head", "table_stride")],
+        *[(name, ctypes.c_int32) for name in (
+            "n_seq", "total_tokens", "max_seqlen", "max_seqlen_k", "n_heads_q", "n_heads_kv", "head_dim", "n_pages",
+            "page_size", "max_pages")],
+        ("softmax_scale", ctypes.c_float),
+        *[(name, ctypes.c_int32) for name in ("window_left", "window_right", "causal")],
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``pe_rotary_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        *[(name, ctypes.c_void_p) for name in ("x", "out", "positions", "inv_freq")],
+        *[(name, ctypes.c_int64) for name in ("x_stride_token", "x_stride_head", "n_tokens")],
+        *[(name, ctypes.c_int32) for name in ("n_heads", "head_dim", "half", "positions_32", "interleaved", "inverse")],
+        ("scale", ctypes.c_float),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    """Mirror of ``pe_append_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        *[(name, ctypes.c_void_p) for name in ("q", "q_out", "k", "v", "k_pages", "v_pages", "page_table", "cu_seqlens",
+                                               "seqlens_k", "inv_freq")],
+        *[(name, ctypes.c_int64) for name in (
+            "q_stride_token", "q_stride_head", "k_stride_token", "k_stride_head", "v_stride_token", "v_stride_head",
+            "kp_stride_page", "kp_stride_token", "kp_stride_head", "vp_stride_page", "vp_stride_token",
+            "vp_stride_head", "table_stride")],
+        *[(name, ctypes.c_int32) for name in ("n_seq", "total_tokens", "n_heads_q", "n_heads_kv", "head_dim", "n_pages",
+                                              "page_size", "max_pages", "half", "interleaved")],
+        ("rope_scale", ctypes.c_float),
+    ]
+
+
 @lru_cache(maxsize=1)
 def library(path: str | None = None) -> ctypes.CDLL:
     """Load the in-tree library once; ``ImportError`` if it is missing or mismatched."""
@@ -121,7 +181,7 @@ def library(path: str | None = None) -> ctypes.CDLL:
         raise ImportError(f"cannot load {lib_path}: {exc}") from exc
     # The version first, then every symbol this package calls: a library built before one was added has
     # the version but not the symbol, and is as stale as one of another version.
-    missing = [name for name in EXPORTED if not hasattr(lib, name)]
+    missing = [name for name in EXPORTED + PAGED_EXPORTED if not hasattr(lib, name)]
     if EXPORTED[0] not in missing:
         lib.pe_attn_abi_version.restype = ctypes.c_int
         lib.pe_attn_abi_version.argtypes = []
@@ -164,6 +224,18 @@ def library(path: str | None = None) -> ctypes.CDLL:
                                       ctypes.c_void_p]
     lib.pe_geglu_fwd.restype = ctypes.c_int
     lib.pe_geglu_fwd.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p]
+    lib.pe_paged_workspace_size.restype = ctypes.c_int
+    lib.pe_paged_workspace_size.argtypes = [ctypes.POINTER(PagedArgs), ctypes.POINTER(ctypes.c_size_t)]
+    lib.pe_paged_attn_fwd.restype = ctypes.c_int
+    lib.pe_paged_attn_fwd.argtypes = [ctypes.POINTER(PagedArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    lib.pe_rotary_fwd.restype = ctypes.c_int
+    lib.pe_rotary_fwd.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.pe_paged_append_fwd.restype = ctypes.c_int
+    lib.pe_paged_append_fwd.argtypes = [ctypes.POINTER(AppendArgs), ctypes.c_void_p]
+    lib.pe_copy_pages.restype = ctypes.c_int
+    lib.pe_copy_pages.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
+                                  ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
+                                  ctypes.c_int32, ctypes.c_void_p]
     return lib
 
 

@@ -1,0 +1,389 @@
+// C ABI of the paged cache (declared in include/pe_paged.h): argument checks, host-side sizing and the
+// launches. Nothing here reads device memory, synchronises or allocates device memory.
+#include "../../include/pe_paged.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+#include <new>
+
+#include "pe_paged_attn.h"
+#include "pe_paged_rope.h"
+
+namespace {
+
+constexpr int64_t kCUs = 256;                      // compute units of an MI355X
+constexpr int64_t kMaxWorkspace = (int64_t)256 << 20;
+constexpr int kMaxChunks = 256;                    // paged_merge_kernel holds a weight per thread
+constexpr int32_t kMaxKeys = 1 << 30;              // key positions and what is added to them stay in 32 bits
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool row_stride(int64_t s) { return s >= 0 && (s & 7) == 0; }
+int launched() { return hipGetLastError() == hipSuccess ? PE_ATTN_OK : PE_ATTN_ELAUNCH; }
+
+// Multiplier and shift of n / d for 0 <= n < 2^31, d >= 2: with 2^(L-1) < d <= 2^L, mul = ceil(2^(31+L) / d)
+// is below 2^32 and exceeds 2^(31+L) / d by less than one, so the product's error stays below 2^31 / 2^(31+L)
+// <= 1 / d and never reaches the next multiple.
+void divider(uint32_t d, uint32_t *mul, uint32_t *shift) {
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    *mul = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+    *shift = l - 1;
+}
+
+int check_pages(int32_t n_pages, int32_t page_size, int32_t max_pages, int64_t table_stride) {
+    if (n_pages < 0 || max_pages < 0 || table_stride < 0 || page_size < PE_PAGED_PAGE_MULTIPLE) return PE_ATTN_EINVAL;
+    if (page_size % PE_PAGED_PAGE_MULTIPLE) return PE_ATTN_EUNSUPPORTED;
+    return PE_ATTN_OK;
+}
+
+// ----------------------------------------------------------------------------- attention
+
+int check_paged(const pe_paged_args *a, bool need_pointers) {
+    if (!a || a->struct_size != sizeof(pe_paged_args)) return PE_ATTN_EINVAL;
+    if (a->dtype != PE_ATTN_DTYPE_BF16) return PE_ATTN_EUNSUPPORTED;
+    if (a->n_seq < 0 || a->total_tokens < 0 || a->max_seqlen < 0 || a->max_seqlen_k < 0) return PE_ATTN_EINVAL;
+    if (a->n_heads_q < 1 || a->n_heads_kv < 1 || a->n_heads_q % a->n_heads_kv) return PE_ATTN_EINVAL;
+    if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return PE_ATTN_EUNSUPPORTED;
+    if (!(a->softmax_scale > 0.0f) || a->softmax_scale > 3e38f) return PE_ATTN_EINVAL;
+    if (a->window_left < -1 || a->window_right < -1) return PE_ATTN_EINVAL;
+    if (a->causal != 0 && a->causal != 1) return PE_ATTN_EINVAL;
+    if (const int status = check_pages(a->n_pages, a->page_size, a->max_pages, a->table_stride)) return status;
+    // 32-bit positions and rows; one dimension of the grid holds tiles x kv heads, another query heads.
+    if (a->max_seqlen_k > kMaxKeys || a->window_left > kMaxKeys || a->window_right > kMaxKeys ||
+        (int64_t)a->max_seqlen * (a->n_heads_q / a->n_heads_kv) > kMaxKeys || a->n_heads_q > 65535)
+        return PE_ATTN_EUNSUPPORTED;
+    if (!need_pointers || a->n_seq == 0 || a->total_tokens == 0) return PE_ATTN_OK;
+    if (!a->q || !a->o || !a->cu_seqlens || !a->seqlens_k) return PE_ATTN_EINVAL;
+    if ((a->n_pages > 0 && (!a->k_pages || !a->v_pages)) || (a->max_pages > 0 && !a->page_table)) return PE_ATTN_EINVAL;
+    const void *ptrs[4] = {a->q, a->k_pages, a->v_pages, a->o};
+    for (const void *p : ptrs)
+        if (!aligned16(p)) return PE_ATTN_EINVAL;
+    const int64_t strides[10] = {a->q_stride_token, a->q_stride_head, a->k_stride_page,  a->k_stride_token, a->k_stride_head,
+                                 a->v_stride_page,  a->v_stride_token, a->v_stride_head, a->o_stride_token, a->o_stride_head};
+    for (int64_t s : strides)
+        if (!row_stride(s)) return PE_ATTN_EINVAL;
+    if (a->k_stride_token < a->head_dim || a->v_stride_token < a->head_dim) return PE_ATTN_EINVAL;
+    if (a->total_tokens > 1 && a->o_stride_token < a->head_dim) return PE_ATTN_EINVAL;
+    // A page's rows and a sequence's output rows are addressed by 32-bit offsets.
+    const int64_t limit = (int64_t)1 << 31;
+    const int64_t page_span = a->k_stride_token > a->v_stride_token ? a->k_stride_token : a->v_stride_token;
+    if (page_span >= limit / 2 / a->page_size) return PE_ATTN_EUNSUPPORTED;
+    const int64_t head_span = a->n_heads_q > 1 ? (a->n_heads_q - 1) * (a->o_stride_head < limit ? a->o_stride_head : limit) : 0;
+    if (a->o_stride_token >= limit || head_span >= limit ||
+        ((int64_t)(a->max_seqlen ? a->max_seqlen - 1 : 0) * a->o_stride_token + head_span + a->head_dim) * 2 >= limit)
+        return PE_ATTN_EUNSUPPORTED;
+    return PE_ATTN_OK;
+}
+
+// How a call runs: rows of a query tile, tiles the grid holds, and the keys split into chunks.
+struct PagedShape {
+    int bm;
+    bool one_tile;
+    int64_t tiles;
+    int32_t chunk;   // keys per workgroup
+    int32_t chunks;  // 1: not split
+};
+
+PagedShape paged_shape(const pe_paged_args *a) {
+    PagedShape s;
+    const int64_t group = a->n_heads_q / a->n_heads_kv, rows = (int64_t)a->max_seqlen * group;
+    s.bm = 128;
+    s.one_tile = rows <= s.bm;
+    const int64_t by_bound = a->n_seq * ((rows + s.bm - 1) / s.bm), by_rows = a->total_tokens * group / s.bm + a->n_seq;
+    s.tiles = s.one_tile ? a->n_seq : (by_bound < by_rows ? by_bound : by_rows);
+    // The most keys a tile reaches (klo is rounded down to a multiple of 64).
+    int64_t reach = a->max_seqlen_k;
+    const int wr = a->causal ? 0 : a->window_right;
+    if (a->window_left >= 0 && wr >= 0) {
+        const int64_t band = (int64_t)a->window_left + wr + (s.bm - 1) / group + 2 + 64;
+        if (band < reach) reach = band;
+    }
+    s.chunk = reach > 64 ? (int32_t)((reach + 63) & ~(int64_t)63) : 64;
+    s.chunks = 1;
+    const int64_t units = s.tiles * a->n_heads_kv, slots = 2 * kCUs;
+    if (units <= 0 || units >= slots || reach <= 256) return s;
+    int64_t want = (2 * slots + units - 1) / units;
+    const int64_t row_bytes = (int64_t)a->total_tokens * a->n_heads_q * (a->head_dim + 2) * 4;
+    if (want > kMaxWorkspace / row_bytes) want = kMaxWorkspace / row_bytes;
+    if (want > kMaxChunks) want = kMaxChunks;
+    if (want < 2) return s;
+    int64_t chunk = ((reach + want - 1) / want + 63) & ~(int64_t)63;
+    if (chunk < 256) chunk = 256;
+    s.chunk = (int32_t)chunk;
+    s.chunks = (int32_t)((reach + chunk - 1) / chunk);
+    return s;
+}
+
+size_t workspace_of(const pe_paged_args *a, const PagedShape &s) {
+    if (s.chunks <= 1) return 0;
+    return (size_t)s.chunks * a->total_tokens * a->n_heads_q * (a->head_dim + 2) * 4;
+}
+
+pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *workspace) {
+    pe::PagedParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = static_cast<const __bf16 *>(a->q);
+    p.k = static_cast<const __bf16 *>(a->k_pages);
+    p.v = static_cast<const __bf16 *>(a->v_pages);
+    p.o = static_cast<__bf16 *>(a->o);
+    p.table = a->page_table;
+    p.cu = a->cu_seqlens;
+    p.lens = a->seqlens_k;
+    p.q_st = a->q_stride_token;
+    p.q_sh = a->q_stride_head;
+    p.k_sp = a->k_stride_page;
+    p.k_st = a->k_stride_token;
+    p.k_sh = a->k_stride_head;
+    p.v_sp = a->v_stride_page;
+    p.v_st = a->v_stride_token;
+    p.v_sh = a->v_stride_head;
+    p.o_st = a->o_stride_token;
+    p.o_sh = a->o_stride_head;
+    p.table_st = a->table_stride;
+    p.n_seq = a->n_seq;
+    p.hq = a->n_heads_q;
+    p.hkv = a->n_heads_kv;
+    p.group = a->n_heads_q / a->n_heads_kv;
+    p.n_pages = a->n_pages;
+    p.page = a->page_size;
+    p.max_pages = a->max_pages;
+    divider((uint32_t)a->page_size, &p.page_mul, &p.page_shift);
+    p.wl = a->window_left;
+    p.wr = a->causal ? 0 : a->window_right;
+    p.max_seqlen = a->max_seqlen;
+    p.max_seqlen_k = a->max_seqlen_k;
+    p.one_tile = s.one_tile ? 1 : 0;
+    p.chunk = s.chunk;
+    p.total_q = a->total_tokens;
+    p.c = a->softmax_scale * pe::kLog2e;
+    if (s.chunks > 1) {
+        p.part_o = static_cast<float *>(workspace);
+        p.part_ml = p.part_o + (int64_t)s.chunks * a->total_tokens * a->n_heads_q * a->head_dim;
+    }
+    return p;
+}
+
+template <int D>
+int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedParams &p, hipStream_t stream) {
+    const int64_t blocks = s.tiles * a->n_heads_kv;
+    if (blocks > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    const dim3 grid((unsigned)blocks, (unsigned)s.chunks);
+    if (s.chunks == 1) {
+        hipLaunchKernelGGL((pe::paged_tile_kernel<D, false>), grid, dim3(256), 0, stream, p);
+        return launched();
+    }
+    hipLaunchKernelGGL((pe::paged_tile_kernel<D, true>), grid, dim3(256), 0, stream, p);
+    if (const int status = launched()) return status;
+    hipLaunchKernelGGL((pe::paged_merge_kernel<D>), dim3((unsigned)a->total_tokens, (unsigned)a->n_heads_q), dim3(256), 0,
+                       stream, p, s.bm, s.chunks);
+    return launched();
+}
+
+// ----------------------------------------------------------------------------- rotary positions
+
+// Tokens and heads of a workgroup: four tokens share a pass over the frequencies, but a call of few tokens
+// takes them one by one, and then spreads their heads, until it has two workgroups per CU.
+void turn_shape(int64_t tokens, int heads, int *per, int *slice) {
+    *per = tokens >= 4 * 2 * kCUs ? pe::kTurnTokens : 1;
+    const int64_t groups = (tokens + *per - 1) / *per;
+    int slices = 1;
+    while (groups * slices < 2 * kCUs && 4 * slices < heads) slices *= 2;
+    *slice = (heads + slices - 1) / slices;
+}
+
+template <typename T, int V>
+int launch_rotary(const pe_rotary_args *a, pe::RotaryParams &p, hipStream_t stream) {
+    const int64_t groups = (a->n_tokens + p.per - 1) / p.per;
+    if (groups > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    const dim3 grid((unsigned)groups, (unsigned)((a->n_heads + p.slice - 1) / p.slice));
+    if (a->interleaved)
+        hipLaunchKernelGGL((pe::rotary_kernel<T, V, true>), grid, dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((pe::rotary_kernel<T, V, false>), grid, dim3(256), 0, stream, p);
+    return launched();
+}
+
+// Whether rows split into units of v elements: whole pieces of the turned and of the copied part.
+bool in_pieces(int v, int d, int half, bool interleaved) {
+    return d % v == 0 && (interleaved ? 2 * half : half) % v == 0 && (d - 2 * half) % v == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pe_paged_workspace_size(const pe_paged_args *args, size_t *bytes) {
+    if (!bytes) return PE_ATTN_EINVAL;
+    if (const int status = check_paged(args, false)) return status;
+    *bytes = args->n_seq && args->total_tokens ? workspace_of(args, paged_shape(args)) : 0;
+    return PE_ATTN_OK;
+}
+
+int pe_paged_attn_fwd(const pe_paged_args *args, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (const int status = check_paged(args, true)) return status;
+    if (args->n_seq == 0 || args->total_tokens == 0 || args->max_seqlen == 0) return PE_ATTN_OK;
+    const PagedShape s = paged_shape(args);
+    const size_t need = workspace_of(args, s);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return PE_ATTN_EWORKSPACE;
+    const pe::PagedParams p = paged_params(args, s, workspace);
+    if (args->head_dim == 64) return launch_paged<64>(args, s, p, stream);
+    if (args->head_dim == 128) return launch_paged<128>(args, s, p, stream);
+    return launch_paged<256>(args, s, p, stream);
+}
+
+int pe_rotary_fwd(const pe_rotary_args *a, hipStream_t stream) {
+    if (!a || a->struct_size != sizeof(pe_rotary_args)) return PE_ATTN_EINVAL;
+    if (a->dtype < PE_ROTARY_BF16 || a->dtype > PE_ROTARY_FP32) return PE_ATTN_EUNSUPPORTED;
+    if (a->n_tokens < 0 || a->n_heads < 0 || a->head_dim < 1 || a->half < 1 || 2 * (int64_t)a->half > a->head_dim)
+        return PE_ATTN_EINVAL;
+    if ((a->interleaved | a->inverse | a->positions_32) & ~1) return PE_ATTN_EINVAL;
+    if (a->half > PE_ROTARY_MAX_PAIRS) return PE_ATTN_EUNSUPPORTED;
+    if (a->n_tokens == 0 || a->n_heads == 0) return PE_ATTN_OK;
+    if (!a->x || !a->out || !a->positions || !a->inv_freq || a->x_stride_token < 0 || a->x_stride_head < 0)
+        return PE_ATTN_EINVAL;
+    pe::RotaryParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.x = a->x;
+    p.out = a->out;
+    p.positions = a->positions;
+    p.inv_freq = a->inv_freq;
+    p.x_st = a->x_stride_token;
+    p.x_sh = a->x_stride_head;
+    p.tokens = a->n_tokens;
+    p.heads = a->n_heads;
+    p.d = a->head_dim;
+    p.half = a->half;
+    p.wide = a->positions_32 ? 0 : 1;
+    p.scale = a->scale;
+    p.sign = a->inverse ? -1.0f : 1.0f;
+    turn_shape(a->n_tokens, a->n_heads, &p.per, &p.slice);
+    if ((int64_t)pe::kTurnTokens * p.slice * a->head_dim > 0x7fffffffLL || (a->n_heads + p.slice - 1) / p.slice > 65535)
+        return PE_ATTN_EUNSUPPORTED;
+    // 16-byte pieces where the rows allow them, else single elements.
+    const int v = a->dtype == PE_ROTARY_FP32 ? 4 : 8;
+    const bool pieces = in_pieces(v, a->head_dim, a->half, a->interleaved) && a->x_stride_token % v == 0 &&
+                        a->x_stride_head % v == 0 && aligned16(a->x) && aligned16(a->out);
+    if (a->dtype == PE_ROTARY_BF16)
+        return pieces ? launch_rotary<__bf16, 8>(a, p, stream) : launch_rotary<__bf16, 1>(a, p, stream);
+    if (a->dtype == PE_ROTARY_FP16)
+        return pieces ? launch_rotary<_Float16, 8>(a, p, stream) : launch_rotary<_Float16, 1>(a, p, stream);
+    return pieces ? launch_rotary<float, 4>(a, p, stream) : launch_rotary<float, 1>(a, p, stream);
+}
+
+int pe_paged_append_fwd(const pe_append_args *a, hipStream_t stream) {
+    if (!a || a->struct_size != sizeof(pe_append_args)) return PE_ATTN_EINVAL;
+    if (a->dtype != PE_ATTN_DTYPE_BF16) return PE_ATTN_EUNSUPPORTED;
+    if (a->n_seq < 0 || a->total_tokens < 0 || a->n_heads_q < 0 || a->n_heads_kv < 1 || a->head_dim < 8 || a->half < 0 ||
+        2 * (int64_t)a->half > a->head_dim || (a->interleaved & ~1) || (a->q != nullptr) != (a->n_heads_q > 0))
+        return PE_ATTN_EINVAL;
+    if (const int status = check_pages(a->n_pages, a->page_size, a->max_pages, a->table_stride)) return status;
+    if (a->head_dim % 8 || a->half > PE_ROTARY_MAX_PAIRS) return PE_ATTN_EUNSUPPORTED;
+    if (a->n_seq == 0 || a->total_tokens == 0) return PE_ATTN_OK;
+    if (!a->k || !a->v || !a->cu_seqlens || !a->seqlens_k || (a->q && !a->q_out) || (a->half && !a->inv_freq))
+        return PE_ATTN_EINVAL;
+    if ((a->n_pages > 0 && (!a->k_pages || !a->v_pages)) || (a->max_pages > 0 && !a->page_table)) return PE_ATTN_EINVAL;
+    const void *ptrs[6] = {a->q, a->q_out, a->k, a->v, a->k_pages, a->v_pages};
+    for (const void *p : ptrs)
+        if (!aligned16(p)) return PE_ATTN_EINVAL;
+    const int64_t strides[12] = {a->q_stride_token, a->q_stride_head,   a->k_stride_token,  a->k_stride_head,
+                                 a->v_stride_token, a->v_stride_head,   a->kp_stride_page,  a->kp_stride_token,
+                                 a->kp_stride_head, a->vp_stride_page,  a->vp_stride_token, a->vp_stride_head};
+    for (int64_t s : strides)
+        if (!row_stride(s)) return PE_ATTN_EINVAL;
+    pe::AppendParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = static_cast<const __bf16 *>(a->q);
+    p.k = static_cast<const __bf16 *>(a->k);
+    p.v = static_cast<const __bf16 *>(a->v);
+    p.q_out = static_cast<__bf16 *>(a->q_out);
+    p.k_pages = static_cast<__bf16 *>(a->k_pages);
+    p.v_pages = static_cast<__bf16 *>(a->v_pages);
+    p.table = a->page_table;
+    p.cu = a->cu_seqlens;
+    p.lens = a->seqlens_k;
+    p.inv_freq = a->inv_freq;
+    p.q_st = a->q_stride_token;
+    p.q_sh = a->q_stride_head;
+    p.k_st = a->k_stride_token;
+    p.k_sh = a->k_stride_head;
+    p.v_st = a->v_stride_token;
+    p.v_sh = a->v_stride_head;
+    p.kp_sp = a->kp_stride_page;
+    p.kp_st = a->kp_stride_token;
+    p.kp_sh = a->kp_stride_head;
+    p.vp_sp = a->vp_stride_page;
+    p.vp_st = a->vp_stride_token;
+    p.vp_sh = a->vp_stride_head;
+    p.table_st = a->table_stride;
+    p.tokens = a->total_tokens;
+    p.n_seq = a->n_seq;
+    p.hq = a->n_heads_q;
+    p.hkv = a->n_heads_kv;
+    p.d = a->head_dim;
+    p.half = a->half;
+    p.n_pages = a->n_pages;
+    p.page = a->page_size;
+    p.max_pages = a->max_pages;
+    divider((uint32_t)a->page_size, &p.page_mul, &p.page_shift);
+    p.scale = a->rope_scale;
+    const int64_t heads = (int64_t)a->n_heads_q + 2 * (int64_t)a->n_heads_kv;
+    if (heads > 65535 || pe::kTurnTokens * heads * a->head_dim > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    turn_shape(a->total_tokens, (int)heads, &p.per, &p.slice);
+    const dim3 grid((unsigned)((a->total_tokens + p.per - 1) / p.per), (unsigned)((heads + p.slice - 1) / p.slice));
+    const bool pieces = in_pieces(8, a->head_dim, a->half, a->interleaved);
+    if (pieces && a->interleaved)
+        hipLaunchKernelGGL((pe::paged_append_kernel<8, true>), grid, dim3(256), 0, stream, p);
+    else if (pieces)
+        hipLaunchKernelGGL((pe::paged_append_kernel<8, false>), grid, dim3(256), 0, stream, p);
+    else if (a->interleaved)
+        hipLaunchKernelGGL((pe::paged_append_kernel<1, true>), grid, dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((pe::paged_append_kernel<1, false>), grid, dim3(256), 0, stream, p);
+    return launched();
+}
+
+int pe_copy_pages(void *const *bases, int32_t n_bases, int64_t page_stride, int64_t page_bytes, int32_t n_pages,
+                  const int32_t *src, const int32_t *dst, int32_t n_pairs, hipStream_t stream) {
+    if (n_bases < 0 || n_pairs < 0 || n_pages < 0 || page_bytes < 0 || page_stride < 0) return PE_ATTN_EINVAL;
+    if ((page_bytes & 15) || (page_stride & 15)) return PE_ATTN_EUNSUPPORTED;
+    if (n_bases == 0 || n_pairs == 0 || page_bytes == 0) return PE_ATTN_OK;
+    if (!bases || !src || !dst || (n_pages > 1 && page_stride < page_bytes)) return PE_ATTN_EINVAL;
+    for (int32_t i = 0; i < n_bases; ++i)
+        if (!bases[i] || !aligned16(bases[i])) return PE_ATTN_EINVAL;
+    unsigned char *seen = new (std::nothrow) unsigned char[(size_t)n_pages + 1]();  // 1: a source, 2: a target
+    if (!seen) return PE_ATTN_EINVAL;
+    bool ok = true;
+    for (int32_t i = 0; ok && i < n_pairs; ++i) {
+        ok = src[i] >= 0 && src[i] < n_pages && dst[i] >= 0 && dst[i] < n_pages;
+        if (ok) seen[src[i]] = 1;
+    }
+    for (int32_t i = 0; ok && i < n_pairs; ++i) {
+        ok = seen[dst[i]] == 0;
+        seen[dst[i]] = 2;
+    }
+    delete[] seen;
+    if (!ok) return PE_ATTN_EINVAL;
+    pe::CopyParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.stride = page_stride;
+    p.pieces = page_bytes / 16;
+    const int64_t blocks = (p.pieces + 256 * pe::kCopyPieces - 1) / (256 * pe::kCopyPieces);
+    if (blocks > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    for (int32_t b = 0; b < n_bases; b += pe::kCopyBases) {
+        const int32_t nb = n_bases - b < pe::kCopyBases ? n_bases - b : pe::kCopyBases;
+        for (int32_t i = 0; i < nb; ++i) p.base[i] = static_cast<char *>(bases[b + i]);
+        for (int32_t c = 0; c < n_pairs; c += pe::kCopyPairs) {
+            const int32_t nc = n_pairs - c < pe::kCopyPairs ? n_pairs - c : pe::kCopyPairs;
+            std::memcpy(p.src, src + c, (size_t)nc * 4);
+            std::memcpy(p.dst, dst + c, (size_t)nc * 4);
+            hipLaunchKernelGGL(pe::copy_pages_kernel, dim3((unsigned)blocks, (unsigned)nc, (unsigned)nb), dim3(256), 0,
+                               stream, p);
+            if (const int status = launched()) return status;
+        }
+    }
+    return PE_ATTN_OK;
+}
+
+}  // extern "C"

@@ -26,8 +26,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <vector>
 
 #include "../../include/pe_attn.h"
+#include "../../include/pe_paged.h"
 
 namespace {
 
@@ -435,6 +437,312 @@ PyObject *attention_qkv(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// rotary(x, positions, inv_freq, interleaved, inverse, scale) -> out, or None. x [tokens, heads, d] with any
+// strides that leave d whole, or contiguous of more axes; positions one per token.
+PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6) {
+        PyErr_SetString(PyExc_TypeError, "rotary takes x, positions, inv_freq, interleaved, inverse and scale");
+        return nullptr;
+    }
+    const double scale = PyFloat_AsDouble(args[5]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    const Tensor *x = nullptr, *pos = nullptr, *freq = nullptr;
+    if (!plain_thread() || !THPVariable_CheckExact(args[0]) || !THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    const at::ScalarType type = THPVariable_Unpack(args[0]).scalar_type();
+    const at::ScalarType index = THPVariable_Unpack(args[1]).scalar_type();
+    const int32_t dtype = type == at::kBFloat16 ? PE_ROTARY_BF16
+                          : type == at::kHalf   ? PE_ROTARY_FP16
+                          : type == at::kFloat  ? PE_ROTARY_FP32
+                                                : 0;
+    if (!dtype || (index != at::kLong && index != at::kInt) || !plain_any(args[0], x, type) ||
+        !plain_any(args[1], pos, index) || !plain_any(args[2], freq, at::kFloat) || x->dim() < 3 || x->numel() == 0 ||
+        freq->dim() != 1 || !freq->is_contiguous() || !pos->is_contiguous())
+        Py_RETURN_NONE;
+    const int64_t dims = x->dim(), d = x->size(dims - 1), heads = x->size(dims - 2), half = freq->numel();
+    const bool rows = dims == 3 && x->stride(2) == 1;
+    if ((!rows && !x->is_contiguous()) || pos->dim() != dims - 2 || pos->sizes() != x->sizes().slice(0, dims - 2) ||
+        half < 1 || half > PE_ROTARY_MAX_PAIRS || 2 * half > d || d > INT32_MAX || heads > INT32_MAX)
+        Py_RETURN_NONE;
+    const auto sizes = x->sizes().vec();
+    const auto options = x->options();
+    const hipStream_t stream = stream_of(*x);
+    pe_rotary_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype;
+    a.x = x->const_data_ptr();
+    a.positions = pos->const_data_ptr();
+    a.inv_freq = static_cast<const float *>(freq->const_data_ptr());
+    a.x_stride_token = rows ? x->stride(0) : heads * d;
+    a.x_stride_head = rows ? x->stride(1) : d;
+    a.n_tokens = x->numel() / (heads * d);
+    a.n_heads = (int32_t)heads;
+    a.head_dim = (int32_t)d;
+    a.half = (int32_t)half;
+    a.positions_32 = index == at::kInt;
+    a.interleaved = args[3] == Py_True;
+    a.inverse = args[4] == Py_True;
+    a.scale = (float)scale;
+    Tensor out;
+    int status;
+    {
+        Unlocked unlocked;
+        out = at::empty(sizes, options);
+        a.out = out.mutable_data_ptr();
+        status = pe_rotary_fwd(&a, stream);
+    }
+    if (failed(status, "pe_rotary_fwd")) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// The pages and what finds them: [n_pages, page_size, heads, d] bf16 twice, int32 table, cu_seqlens, seqlens_k.
+struct Pages {
+    const Tensor *k = nullptr, *v = nullptr, *table = nullptr, *cu = nullptr, *lens = nullptr;
+
+    static bool rows(PyObject *obj, const Tensor *&out) {
+        return plain_any(obj, out, at::kBFloat16) && out->dim() == 4 && out->stride(3) == 1 && aligned16(*out) &&
+               out->stride(0) % 8 == 0 && out->stride(1) % 8 == 0 && out->stride(2) % 8 == 0;
+    }
+    bool parse(PyObject *const *a) {
+        if (!rows(a[0], k) || !rows(a[1], v) || k->sizes() != v->sizes() || !plain_any(a[2], table, at::kInt) ||
+            table->dim() != 2 || !plain_bounds(a[3], cu) || !plain_bounds(a[4], lens))
+            return false;
+        const int64_t n = cu->numel() - 1;
+        if (n < 1 || n > INT32_MAX || lens->numel() != n || table->size(0) != n || table->size(1) > INT32_MAX ||
+            (table->size(1) > 1 && table->stride(1) != 1))
+            return false;
+        for (int i = 0; i < 4; ++i)
+            if (k->size(i) > INT32_MAX) return false;
+        return k->size(1) >= PE_PAGED_PAGE_MULTIPLE && k->size(1) % PE_PAGED_PAGE_MULTIPLE == 0 && k->size(2) >= 1;
+    }
+};
+
+// paged_attention(q, k_pages, v_pages, table, cu, lens, max_seqlen, max_seqlen_k, scale, window_left, window_right,
+// causal) -> out, or None
+PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 12) {
+        PyErr_SetString(PyExc_TypeError, "paged_attention takes its six tensors and six options");
+        return nullptr;
+    }
+    const int at_int[4] = {6, 7, 9, 10};
+    int64_t ints[4];
+    bool fits = true;
+    for (int i = 0; i < 4; ++i) {
+        ints[i] = PyLong_AsLongLong(args[at_int[i]]);
+        if (ints[i] == -1 && PyErr_Occurred()) return nullptr;
+        fits = fits && ints[i] >= INT32_MIN && ints[i] <= INT32_MAX;
+    }
+    const double scale = PyFloat_AsDouble(args[8]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    const Tensor *q = nullptr;
+    Pages pages;
+    if (!fits || !plain_thread() || !plain_rows(args[0], q) || !pages.parse(args + 1)) Py_RETURN_NONE;
+    const Tensor &k = *pages.k, &v = *pages.v;
+    if (q->size(2) != k.size(3) || q->size(1) < 1 || q->size(1) % k.size(2) || q->size(0) == 0 || q->size(0) > INT32_MAX ||
+        q->size(1) > INT32_MAX)
+        Py_RETURN_NONE;
+    pe_paged_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = PE_ATTN_DTYPE_BF16;
+    a.q = q->const_data_ptr();
+    a.k_pages = k.const_data_ptr();
+    a.v_pages = v.const_data_ptr();
+    a.page_table = static_cast<const int32_t *>(pages.table->const_data_ptr());
+    a.cu_seqlens = static_cast<const int32_t *>(pages.cu->const_data_ptr());
+    a.seqlens_k = static_cast<const int32_t *>(pages.lens->const_data_ptr());
+    a.q_stride_token = q->stride(0);
+    a.q_stride_head = q->stride(1);
+    a.k_stride_page = k.stride(0);
+    a.k_stride_token = k.stride(1);
+    a.k_stride_head = k.stride(2);
+    a.v_stride_page = v.stride(0);
+    a.v_stride_token = v.stride(1);
+    a.v_stride_head = v.stride(2);
+    a.o_stride_head = q->size(2);
+    a.o_stride_token = q->size(1) * q->size(2);
+    a.table_stride = pages.table->stride(0);
+    a.n_seq = (int32_t)pages.lens->numel();
+    a.total_tokens = (int32_t)q->size(0);
+    a.max_seqlen = (int32_t)ints[0];
+    a.max_seqlen_k = (int32_t)ints[1];
+    a.n_heads_q = (int32_t)q->size(1);
+    a.n_heads_kv = (int32_t)k.size(2);
+    a.head_dim = (int32_t)q->size(2);
+    a.n_pages = (int32_t)k.size(0);
+    a.page_size = (int32_t)k.size(1);
+    a.max_pages = (int32_t)pages.table->size(1);
+    a.softmax_scale = (float)scale;
+    a.window_left = (int32_t)ints[2];
+    a.window_right = (int32_t)ints[3];
+    a.causal = args[11] == Py_True;
+    const auto sizes = q->sizes().vec();
+    const auto options = q->options();
+    const hipStream_t stream = stream_of(*q);
+    Tensor out, workspace;
+    const char *what = "pe_paged_workspace_size";
+    int status;
+    {
+        Unlocked unlocked;
+        out = at::empty(sizes, options);
+        a.o = out.mutable_data_ptr();
+        size_t bytes = 0;
+        status = pe_paged_workspace_size(&a, &bytes);
+        if (status == PE_ATTN_OK) {
+            if (bytes) workspace = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+            what = "pe_paged_attn_fwd";
+            status = pe_paged_attn_fwd(&a, bytes ? workspace.mutable_data_ptr() : nullptr, bytes, stream);
+        }
+    }
+    if (failed(status, what)) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_append(q or None, k, v, k_pages, v_pages, table, cu, lens, inv_freq or None, interleaved, rope_scale) -> the
+// rotated q (True without q), or None
+PyObject *paged_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 11) {
+        PyErr_SetString(PyExc_TypeError, "paged_append takes nine tensors, interleaved and rope_scale");
+        return nullptr;
+    }
+    const double scale = PyFloat_AsDouble(args[10]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    const bool queries = args[0] != Py_None, turns = args[8] != Py_None;
+    const Tensor *q = nullptr, *k = nullptr, *v = nullptr, *freq = nullptr;
+    Pages pages;
+    if (!plain_thread() || (queries && !plain_rows(args[0], q)) || !plain_rows(args[1], k) || !plain_rows(args[2], v) ||
+        !pages.parse(args + 3) || (turns && !plain_any(args[8], freq, at::kFloat)))
+        Py_RETURN_NONE;
+    const int64_t d = k->size(2), half = turns ? freq->numel() : 0;
+    if (k->sizes() != v->sizes() || k->size(1) != pages.k->size(2) || d != pages.k->size(3) || d % 8 || k->size(0) == 0 ||
+        k->size(0) > INT32_MAX ||
+        (queries && (q->size(0) != k->size(0) || q->size(2) != d || q->size(1) < 1 || q->size(1) > INT32_MAX)) ||
+        (turns && (freq->dim() != 1 || !freq->is_contiguous() || half < 1 || half > PE_ROTARY_MAX_PAIRS || 2 * half > d)))
+        Py_RETURN_NONE;
+    pe_append_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = PE_ATTN_DTYPE_BF16;
+    a.k = k->const_data_ptr();
+    a.v = v->const_data_ptr();
+    a.page_table = static_cast<const int32_t *>(pages.table->const_data_ptr());
+    a.cu_seqlens = static_cast<const int32_t *>(pages.cu->const_data_ptr());
+    a.seqlens_k = static_cast<const int32_t *>(pages.lens->const_data_ptr());
+    a.inv_freq = turns ? static_cast<const float *>(freq->const_data_ptr()) : nullptr;
+    a.k_stride_token = k->stride(0);
+    a.k_stride_head = k->stride(1);
+    a.v_stride_token = v->stride(0);
+    a.v_stride_head = v->stride(1);
+    a.kp_stride_page = pages.k->stride(0);
+    a.kp_stride_token = pages.k->stride(1);
+    a.kp_stride_head = pages.k->stride(2);
+    a.vp_stride_page = pages.v->stride(0);
+    a.vp_stride_token = pages.v->stride(1);
+    a.vp_stride_head = pages.v->stride(2);
+    a.table_stride = pages.table->stride(0);
+    a.n_seq = (int32_t)pages.lens->numel();
+    a.total_tokens = (int32_t)k->size(0);
+    a.n_heads_kv = (int32_t)k->size(1);
+    a.head_dim = (int32_t)d;
+    a.n_pages = (int32_t)pages.k->size(0);
+    a.page_size = (int32_t)pages.k->size(1);
+    a.max_pages = (int32_t)pages.table->size(1);
+    a.half = (int32_t)half;
+    a.interleaved = args[9] == Py_True;
+    a.rope_scale = (float)scale;
+    a.k_pages = pages.k->mutable_data_ptr();
+    a.v_pages = pages.v->mutable_data_ptr();
+    const auto options = k->options();
+    const hipStream_t stream = stream_of(*k);
+    int64_t sizes[3] = {0, 0, 0};
+    if (queries) {
+        a.q = q->const_data_ptr();
+        a.q_stride_token = q->stride(0);
+        a.q_stride_head = q->stride(1);
+        a.n_heads_q = (int32_t)q->size(1);
+        for (int i = 0; i < 3; ++i) sizes[i] = q->size(i);
+    }
+    Tensor out;
+    int status;
+    {
+        Unlocked unlocked;
+        if (queries) {
+            out = at::empty(at::IntArrayRef(sizes, 3), options);
+            a.q_out = out.mutable_data_ptr();
+        }
+        status = pe_paged_append_fwd(&a, stream);
+    }
+    if (failed(status, "pe_paged_append_fwd")) return nullptr;
+    if (!queries) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// Python integers of a list into `out`; false, with no exception left, for anything else.
+bool page_list(PyObject *list, std::vector<int32_t> &out) {
+    if (!PyList_CheckExact(list)) return false;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    out.resize(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const int64_t x = PyLong_AsLongLong(PyList_GET_ITEM(list, i));
+        if (x == -1 && PyErr_Occurred()) {
+            PyErr_Clear();
+            return false;
+        }
+        if (x < 0 || x > INT32_MAX) return false;
+        out[i] = (int32_t)x;
+    }
+    return true;
+}
+
+// copy_pages([caches], [src], [dst]) -> True, or None. Contiguous caches of one shape and type.
+PyObject *copy_pages(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3 || !PyList_CheckExact(args[0])) {
+        PyErr_SetString(PyExc_TypeError, "copy_pages takes lists of caches, sources and targets");
+        return nullptr;
+    }
+    const Py_ssize_t count = PyList_GET_SIZE(args[0]);
+    std::vector<int32_t> src, dst;
+    if (!plain_thread() || count < 1 || !page_list(args[1], src) || !page_list(args[2], dst) || src.size() != dst.size() ||
+        src.size() > INT32_MAX)
+        Py_RETURN_NONE;
+    std::vector<void *> bases;
+    int64_t pages = 0, page_bytes = 0;
+    hipStream_t stream = nullptr;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        PyObject *obj = PyList_GET_ITEM(args[0], i);
+        const Tensor *t = nullptr;
+        if (!THPVariable_CheckExact(obj) || !plain_any(obj, t, THPVariable_Unpack(obj).scalar_type()) || t->dim() < 4 ||
+            !t->is_contiguous() || t->numel() == 0)
+            Py_RETURN_NONE;
+        const int64_t dims = t->dim(), at = t->size(dims - 4);
+        const int64_t bytes = t->size(dims - 3) * t->size(dims - 2) * t->size(dims - 1) * (int64_t)t->element_size();
+        if (i && (at != pages || bytes != page_bytes)) Py_RETURN_NONE;
+        pages = at;
+        page_bytes = bytes;
+        const int64_t caches = (int64_t)t->nbytes() / (at * bytes);
+        if (pages > INT32_MAX || (int64_t)bases.size() + caches > INT32_MAX) Py_RETURN_NONE;
+        char *base = static_cast<char *>(t->mutable_data_ptr());
+        for (int64_t c = 0; c < caches; ++c) bases.push_back(base + c * at * bytes);
+        stream = stream_of(*t);
+    }
+    int status;
+    {
+        Unlocked unlocked;
+        status = pe_copy_pages(bases.data(), (int32_t)bases.size(), page_bytes, page_bytes, (int32_t)pages, src.data(),
+                               dst.data(), (int32_t)src.size(), stream);
+    }
+    if (failed(status, "pe_copy_pages")) return nullptr;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 #define PE_FASTCALL(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 
 PyMethodDef methods[] = {
@@ -448,6 +756,13 @@ PyMethodDef methods[] = {
     {"attention_qkv", PE_FASTCALL(attention_qkv),
      "attention_qkv(qkv, h, d, cu, cos, sin, max_seqlen, window_left, window_right, causal, short_max, max_seqlen_k, "
      "band_kernel, min_seqlen, scale, args) -> out, (out, stream) or None"},
+    {"rotary", PE_FASTCALL(rotary), "rotary(x, positions, inv_freq, interleaved, inverse, scale) -> out or None"},
+    {"paged_attention", PE_FASTCALL(paged_attention),
+     "paged_attention(q, k_pages, v_pages, table, cu, lens, max_seqlen, max_seqlen_k, scale, window_left, window_right, "
+     "causal) -> out or None"},
+    {"paged_append", PE_FASTCALL(paged_append),
+     "paged_append(q, k, v, k_pages, v_pages, table, cu, lens, inv_freq, interleaved, rope_scale) -> q, True or None"},
+    {"copy_pages", PE_FASTCALL(copy_pages), "copy_pages(caches, src, dst) -> True or None"},
     {nullptr, nullptr, 0, nullptr},
 };
 
