@@ -15,7 +15,6 @@ namespace {
 
 constexpr int64_t kCUs = 256;                      // compute units of an MI355X
 constexpr int64_t kMaxWorkspace = (int64_t)256 << 20;
-constexpr int kMaxChunks = 256;                    // paged_merge_kernel holds a weight per thread
 constexpr int32_t kMaxKeys = 1 << 30;              // key positions and what is added to them stay in 32 bits
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -77,7 +76,8 @@ int check_paged(const pe_paged_args *a, bool need_pointers) {
     return PE_ATTN_OK;
 }
 
-// How a call runs: rows of a query tile, tiles the grid holds, and the keys split into chunks.
+// How a call runs: rows of a query tile (16 or 32: paged_row_kernel, 128: paged_tile_kernel), tiles the
+// grid holds, and the keys split into chunks.
 struct PagedShape {
     int bm;
     bool one_tile;
@@ -89,7 +89,7 @@ struct PagedShape {
 PagedShape paged_shape(const pe_paged_args *a) {
     PagedShape s;
     const int64_t group = a->n_heads_q / a->n_heads_kv, rows = (int64_t)a->max_seqlen * group;
-    s.bm = 128;
+    s.bm = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     s.one_tile = rows <= s.bm;
     const int64_t by_bound = a->n_seq * ((rows + s.bm - 1) / s.bm), by_rows = a->total_tokens * group / s.bm + a->n_seq;
     s.tiles = s.one_tile ? a->n_seq : (by_bound < by_rows ? by_bound : by_rows);
@@ -102,15 +102,19 @@ PagedShape paged_shape(const pe_paged_args *a) {
     }
     s.chunk = reach > 64 ? (int32_t)((reach + 63) & ~(int64_t)63) : 64;
     s.chunks = 1;
-    const int64_t units = s.tiles * a->n_heads_kv, slots = 2 * kCUs;
-    if (units <= 0 || units >= slots || reach <= 256) return s;
-    int64_t want = (2 * slots + units - 1) / units;
+    // Workgroups the chip holds at once: two per CU. Calls of fewer (sequence, kv head) tiles split their
+    // keys; tiles of few rows until each slot has about four workgroups, since the sequences' lengths differ
+    // and the last ones to end leave the chip idle.
+    const int64_t units = s.tiles * a->n_heads_kv, slots = 2 * kCUs, goal = s.bm < 128 ? 8 * slots : 2 * slots;
+    const int64_t least = s.bm < 128 ? 128 : 256;
+    if (units <= 0 || units >= (s.bm < 128 ? goal : slots) || reach <= least) return s;
+    int64_t want = (goal + units - 1) / units;
     const int64_t row_bytes = (int64_t)a->total_tokens * a->n_heads_q * (a->head_dim + 2) * 4;
     if (want > kMaxWorkspace / row_bytes) want = kMaxWorkspace / row_bytes;
-    if (want > kMaxChunks) want = kMaxChunks;
+    if (want > pe::kMaxChunks) want = pe::kMaxChunks;
     if (want < 2) return s;
     int64_t chunk = ((reach + want - 1) / want + 63) & ~(int64_t)63;
-    if (chunk < 256) chunk = 256;
+    if (chunk < least) chunk = least;
     s.chunk = (int32_t)chunk;
     s.chunks = (int32_t)((reach + chunk - 1) / chunk);
     return s;
@@ -165,17 +169,26 @@ pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *
     return p;
 }
 
+template <int D, bool SPLIT>
+int launch_tiles(const PagedShape &s, const pe::PagedParams &p, dim3 grid, hipStream_t stream) {
+    // Waves and stages of a row workgroup: 64 KB of LDS, two workgroups per CU (head_dim 64: 48 KB, three).
+    constexpr int NW = D == 256 ? 1 : 2, NS = D == 64 ? 3 : 2;
+    if (s.bm == 16)
+        hipLaunchKernelGGL((pe::paged_row_kernel<D, 1, NW, NS, SPLIT>), grid, dim3(64 * NW), 0, stream, p);
+    else if (s.bm == 32)
+        hipLaunchKernelGGL((pe::paged_row_kernel<D, 2, NW, NS, SPLIT>), grid, dim3(64 * NW), 0, stream, p);
+    else
+        hipLaunchKernelGGL((pe::paged_tile_kernel<D, SPLIT>), grid, dim3(256), 0, stream, p);
+    return launched();
+}
+
 template <int D>
 int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedParams &p, hipStream_t stream) {
     const int64_t blocks = s.tiles * a->n_heads_kv;
     if (blocks > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
     const dim3 grid((unsigned)blocks, (unsigned)s.chunks);
-    if (s.chunks == 1) {
-        hipLaunchKernelGGL((pe::paged_tile_kernel<D, false>), grid, dim3(256), 0, stream, p);
-        return launched();
-    }
-    hipLaunchKernelGGL((pe::paged_tile_kernel<D, true>), grid, dim3(256), 0, stream, p);
-    if (const int status = launched()) return status;
+    if (s.chunks == 1) return launch_tiles<D, false>(s, p, grid, stream);
+    if (const int status = launch_tiles<D, true>(s, p, grid, stream)) return status;
     hipLaunchKernelGGL((pe::paged_merge_kernel<D>), dim3((unsigned)a->total_tokens, (unsigned)a->n_heads_q), dim3(256), 0,
                        stream, p, s.bm, s.chunks);
     return launched();

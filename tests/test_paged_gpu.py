@@ -123,6 +123,32 @@ def test_masked_keys_may_hold_anything(pe, heads, junk):
     oracle.assert_within(got[40:], want[40:], bound[40:])
 
 
+@pytest.mark.parametrize("heads", [(32, 8, 128), (8, 2, 256), (12, 12, 64)])
+@pytest.mark.parametrize("new", [40, 4])
+def test_infinite_values_reach_the_rows_that_attend_to_them(pe, heads, new):
+    """Infinities and NaN in single dims of v: rows that reach the key take them there, other rows and dims
+    stay as the finite values give them."""
+    hq, hkv, d = heads
+    gen = torch.Generator().manual_seed(12)
+    keys = [90]
+    k, v, table = _cache(keys, 16, hkv, d, gen)
+    clean = v.clone()
+    junk = {(89, 3): float("inf"), (89, 20): float("nan"), (87, 33): -float("inf"), (87, 3): float("inf")}
+    for (j, dim), x in junk.items():
+        v[table[0, j // 16], j % 16, 0, dim] = x
+        clean[table[0, j // 16], j % 16, 0, dim] = 0.0
+    q = torch.randn(new, hq, d, generator=gen).bfloat16()
+    want, bound = oracle.attention(q, k, clean, table, [new], keys)
+    got = _run(pe, q, k, v, table, [new], keys).cpu()
+    mine = slice(0, hq // hkv)  # the query heads of kv head 0
+    at = torch.arange(90 - new, 90)
+    assert torch.isnan(got[at >= 89][:, mine, 20]).all()
+    assert (got[at >= 87][:, mine, 3] == float("inf")).all() and (got[at >= 87][:, mine, 33] == -float("inf")).all()
+    for dim, first in ((20, 89), (3, 87), (33, 87)):
+        got[at >= first, mine, dim] = want[at >= first, mine, dim].bfloat16()
+    oracle.assert_within(got, want, bound)
+
+
 def test_unmapped_pages_are_masked(pe):
     """-1, ids past the cache and far negative ones: their keys do not exist, for single tokens and chunks."""
     for heads in [(32, 8, 128), (8, 2, 256), (12, 12, 64)]:
@@ -208,7 +234,7 @@ def test_rows_of_no_sequence_are_left_as_they_were(pe, split, longest):
     lib = _lib.library()
     hq, hkv, d, page = 8, 2, 128, 16
     gen = torch.Generator().manual_seed(8)
-    bound_k = 1500 if split else 250
+    bound_k = 1500 if split else 125
     new = [2, longest + 1, 2, 2, 2, longest]  # the second has too many rows
     lens = [100, 100, bound_k + 1, 90, -1, 120]  # the third too many keys, the fifth a negative count
     columns = (bound_k + page) // page
