@@ -14,7 +14,6 @@
 namespace {
 
 constexpr int64_t kCUs = 256;                      // compute units of an MI355X
-constexpr int64_t kMaxWorkspace = (int64_t)256 << 20;
 constexpr int32_t kMaxKeys = 1 << 30;              // key positions and what is added to them stay in 32 bits
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -76,54 +75,63 @@ int check_paged(const pe_paged_args *a, bool need_pointers) {
     return PE_ATTN_OK;
 }
 
-// How a call runs: rows of a query tile (16 or 32: paged_row_kernel, 128: paged_tile_kernel), tiles the
-// grid holds, and the keys split into chunks.
+// How a call runs: paged_row_kernel for sequences of at most `few` rows (times the heads of a kv head) when
+// row_blocks > 0, paged_tile_kernel for the others when tiles > 0.
 struct PagedShape {
-    int bm;
-    bool one_tile;
-    int64_t tiles;
-    int32_t chunk;   // keys per workgroup
-    int32_t chunks;  // 1: not split
+    int32_t few;
+    int row_blocks;   // of 16 rows
+    int32_t workers;  // waves per kv head
+    int64_t tiles;    // items per kv head, at most
+    int32_t goal;     // workgroups its keys are split for, 0: not split
+    int64_t run_slots, tile_slots;  // rows of parts, at most
 };
+
+// Waves that run at once on a CU: as many as divide among its SIMDs and have their stages in its 160 KB of LDS
+// (head_dim 64: 16 KB each, 128: 48 KB, 256: 64 KB). At head_dim 128, 64 decoding users of U{512..8192} keys, 32:8
+// heads: three waves of three stages 213 us, four of two 213 us (of five rows each 255 and 278 us), five of two
+// 258 us (a fifth wave per CU waits for a second round), two of four 220 us; 64 users of 12 heads of 64: eight of
+// two stages 161 us, six of three 169 us, ten of two 182 us.
+int row_waves(int head_dim) { return head_dim == 64 ? 8 : head_dim == 128 ? 3 : 2; }
 
 PagedShape paged_shape(const pe_paged_args *a) {
     PagedShape s;
+    std::memset(&s, 0, sizeof(s));
     const int64_t group = a->n_heads_q / a->n_heads_kv, rows = (int64_t)a->max_seqlen * group;
-    s.bm = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
-    s.one_tile = rows <= s.bm;
-    const int64_t by_bound = a->n_seq * ((rows + s.bm - 1) / s.bm), by_rows = a->total_tokens * group / s.bm + a->n_seq;
-    s.tiles = s.one_tile ? a->n_seq : (by_bound < by_rows ? by_bound : by_rows);
-    // The most keys a tile reaches (klo is rounded down to a multiple of 64).
-    int64_t reach = a->max_seqlen_k;
-    const int wr = a->causal ? 0 : a->window_right;
-    if (a->window_left >= 0 && wr >= 0) {
-        const int64_t band = (int64_t)a->window_left + wr + (s.bm - 1) / group + 2 + 64;
-        if (band < reach) reach = band;
+    const int64_t n = a->n_seq, hkv = a->n_heads_kv;
+    // A sequence's steps of 32 keys (one at least), summed over the sequences in 32 bits.
+    const int64_t steps = (a->max_seqlen_k > 32 ? ((int64_t)a->max_seqlen_k + 31) / 32 : 1) * n;
+    const bool uneven = n > 1 && 2 * (int64_t)a->total_tokens < n * a->max_seqlen;  // some sequences are short
+    if ((rows <= 32 || (uneven && group <= 16)) && steps < (int64_t)1 << 30) {
+        s.few = rows > 16 && rows <= 32 ? 32 : 16;
+        s.row_blocks = s.few / 16;
+        int64_t workers = row_waves(a->head_dim) * kCUs / hkv;
+        const int64_t most = (steps + pe::kRunSteps - 1) / pe::kRunSteps;
+        if (workers > most) workers = most;
+        if (workers > pe::kMaxParts) workers = pe::kMaxParts;
+        s.workers = (int32_t)(workers < 1 ? 1 : workers);
+        if (s.workers > 1) s.run_slots = s.workers * hkv * 2 * s.few;
+        if (rows <= 32) return s;
     }
-    s.chunk = reach > 64 ? (int32_t)((reach + 63) & ~(int64_t)63) : 64;
-    s.chunks = 1;
-    // Workgroups the chip holds at once: two per CU. Calls of fewer (sequence, kv head) tiles split their
-    // keys; tiles of few rows until each slot has about four workgroups, since the sequences' lengths differ
-    // and the last ones to end leave the chip idle.
-    const int64_t units = s.tiles * a->n_heads_kv, slots = 2 * kCUs, goal = s.bm < 128 ? 8 * slots : 2 * slots;
-    const int64_t least = s.bm < 128 ? 128 : 256;
-    if (units <= 0 || units >= (s.bm < 128 ? goal : slots) || reach <= least) return s;
-    int64_t want = (goal + units - 1) / units;
-    const int64_t row_bytes = (int64_t)a->total_tokens * a->n_heads_q * (a->head_dim + 2) * 4;
-    if (want > kMaxWorkspace / row_bytes) want = kMaxWorkspace / row_bytes;
-    if (want > pe::kMaxChunks) want = pe::kMaxChunks;
-    if (want < 2) return s;
-    int64_t chunk = ((reach + want - 1) / want + 63) & ~(int64_t)63;
-    if (chunk < least) chunk = least;
-    s.chunk = (int32_t)chunk;
-    s.chunks = (int32_t)((reach + chunk - 1) / chunk);
+    // Tiles: at least as many as the rows fill, at most one more for every sequence with any.
+    const int64_t fill = (a->total_tokens * group + pe::kTileRows - 1) / pe::kTileRows;
+    int64_t with = a->total_tokens * group / (s.few + 1);
+    if (with > n) with = n;
+    s.tiles = fill + with;
+    // Two workgroups per CU run at once (head_dim 256: one, for its registers). Calls of fewer tiles split
+    // their keys into about twice as many items.
+    const int64_t at_once = (a->head_dim == 256 ? 1 : 2) * kCUs;
+    if (fill * hkv < at_once && a->max_seqlen_k > 64 * pe::kChunkSteps) {
+        s.goal = (int32_t)(2 * at_once);
+        // Chunks hold at least 1 / goal of the work, so there are at most goal whole ones; a tile that is split
+        // has at most one that is not whole beside one that is.
+        const int64_t longest = (a->max_seqlen_k + 64 * pe::kChunkSteps - 1) / (64 * pe::kChunkSteps) * s.tiles * hkv;
+        s.tile_slots = (longest < 2 * s.goal ? longest : 2 * s.goal) * pe::kTileRows;
+        s.tiles += (s.goal + hkv - 1) / hkv;
+    }
     return s;
 }
 
-size_t workspace_of(const pe_paged_args *a, const PagedShape &s) {
-    if (s.chunks <= 1) return 0;
-    return (size_t)s.chunks * a->total_tokens * a->n_heads_q * (a->head_dim + 2) * 4;
-}
+size_t workspace_of(const pe_paged_args *a, const PagedShape &s) { return (size_t)(s.run_slots + s.tile_slots) * (a->head_dim + 2) * 4; }
 
 pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *workspace) {
     pe::PagedParams p;
@@ -158,40 +166,56 @@ pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *
     p.wr = a->causal ? 0 : a->window_right;
     p.max_seqlen = a->max_seqlen;
     p.max_seqlen_k = a->max_seqlen_k;
-    p.one_tile = s.one_tile ? 1 : 0;
-    p.chunk = s.chunk;
+    p.few = s.few;
+    p.workers = s.workers;
+    p.goal = s.goal;
+    p.tile_slots = s.run_slots;
     p.total_q = a->total_tokens;
     p.c = a->softmax_scale * pe::kLog2e;
-    if (s.chunks > 1) {
-        p.part_o = static_cast<float *>(workspace);
-        p.part_ml = p.part_o + (int64_t)s.chunks * a->total_tokens * a->n_heads_q * a->head_dim;
-    }
+    p.part_o = static_cast<float *>(workspace);
+    if (workspace) p.part_ml = p.part_o + (s.run_slots + s.tile_slots) * a->head_dim;
     return p;
 }
 
-template <int D, bool SPLIT>
-int launch_tiles(const PagedShape &s, const pe::PagedParams &p, dim3 grid, hipStream_t stream) {
-    // Waves and stages of a row workgroup: 64 KB of LDS, two workgroups per CU (head_dim 64: 48 KB, three).
-    constexpr int NW = D == 256 ? 1 : 2, NS = D == 64 ? 3 : 2;
-    if (s.bm == 16)
-        hipLaunchKernelGGL((pe::paged_row_kernel<D, 1, NW, NS, SPLIT>), grid, dim3(64 * NW), 0, stream, p);
-    else if (s.bm == 32)
-        hipLaunchKernelGGL((pe::paged_row_kernel<D, 2, NW, NS, SPLIT>), grid, dim3(64 * NW), 0, stream, p);
+template <int D, bool RUNS, bool TILES>
+int launch_merge(const pe_paged_args *a, const pe::PagedParams &p, hipStream_t stream) {
+    // A wave per row and some heads once the rows fill the chip, else a workgroup for 64 dims of each.
+    const int64_t items = (int64_t)a->total_tokens * a->n_heads_q;
+    constexpr int heads = 64 / (D / 4);
+    const int64_t waves = (int64_t)a->total_tokens * ((a->n_heads_q + heads - 1) / heads);
+    if (items >= 2 * kCUs)
+        hipLaunchKernelGGL((pe::paged_merge_kernel<D, RUNS, TILES>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream,
+                           p);
     else
-        hipLaunchKernelGGL((pe::paged_tile_kernel<D, SPLIT>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((pe::paged_merge_long_kernel<D, RUNS, TILES>),
+                           dim3((unsigned)a->total_tokens, (unsigned)a->n_heads_q, D / 64), dim3(256), 0, stream, p);
     return launched();
 }
 
 template <int D>
 int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedParams &p, hipStream_t stream) {
     const int64_t blocks = s.tiles * a->n_heads_kv;
-    if (blocks > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
-    const dim3 grid((unsigned)blocks, (unsigned)s.chunks);
-    if (s.chunks == 1) return launch_tiles<D, false>(s, p, grid, stream);
-    if (const int status = launch_tiles<D, true>(s, p, grid, stream)) return status;
-    hipLaunchKernelGGL((pe::paged_merge_kernel<D>), dim3((unsigned)a->total_tokens, (unsigned)a->n_heads_q), dim3(256), 0,
-                       stream, p, s.bm, s.chunks);
-    return launched();
+    if (blocks > 0x7fffffffLL || (int64_t)a->total_tokens * a->n_heads_q > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    if (s.row_blocks) {
+        constexpr int NS = D == 128 ? 3 : 2;
+        const dim3 grid((unsigned)(s.workers * a->n_heads_kv));
+        if (s.row_blocks == 1)
+            hipLaunchKernelGGL((pe::paged_row_kernel<D, 1, NS>), grid, dim3(64), 0, stream, p);
+        else
+            hipLaunchKernelGGL((pe::paged_row_kernel<D, 2, NS>), grid, dim3(64), 0, stream, p);
+        if (const int status = launched()) return status;
+    }
+    if (s.tiles) {
+        if (s.goal)
+            hipLaunchKernelGGL((pe::paged_tile_kernel<D, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((pe::paged_tile_kernel<D, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        if (const int status = launched()) return status;
+    }
+    if (s.run_slots && s.tile_slots) return launch_merge<D, true, true>(a, p, stream);
+    if (s.run_slots) return launch_merge<D, true, false>(a, p, stream);
+    if (s.tile_slots) return launch_merge<D, false, true>(a, p, stream);
+    return PE_ATTN_OK;
 }
 
 // ----------------------------------------------------------------------------- rotary positions

@@ -26,11 +26,13 @@ struct PagedParams {
     uint32_t page_mul, page_shift;  // n / page = (n * page_mul >> 32) >> page_shift for 0 <= n < 2^31
     int32_t wl, wr;                 // window (-1: unbounded); causal folded into wr = 0
     int32_t max_seqlen, max_seqlen_k;
-    int32_t one_tile;               // 1: every sequence has at most one query tile, its own
-    int32_t chunk;                  // keys per workgroup along grid y
+    int32_t few;                    // sequences of at most this many rows are paged_row_kernel's (0: none)
+    int32_t workers;                // its waves per kv head
+    int32_t goal;                   // workgroups that paged_tile_kernel's items should come to, over the kv heads
     int32_t total_q;
     float c;                        // softmax_scale * log2(e)
-    float *part_o, *part_ml;        // split calls: [chunks][total_q][hq][D] and [..][2], fp32
+    int64_t tile_slots;             // first slot of paged_tile_kernel's parts
+    float *part_o, *part_ml;        // split rows' parts [slots][D] and their maxima and sums [slots][2], fp32
 };
 
 __device__ __forceinline__ int page_of(const PagedParams &p, int key) {
@@ -46,65 +48,33 @@ __device__ __forceinline__ PageIds page_ids_of(const PagedParams &p, int seq) {
     return (PageIds)(uintptr_t)(p.table + (int64_t)seq * p.table_st);
 }
 
-// A query tile of `bm` rows: sequence, first row, rows of the sequence, key position of its token 0.
-struct PagedTile {
-    int seq, row0, rows, start, lk, off;
-    bool valid;
+// 64 sequences from `base` on, one per lane: the new rows (times the heads of a kv head) of those that the call
+// serves, 0 for the others, and their bounds.
+struct Lanes {
+    int start, rows, lk;
 };
 
-// The sequence's bounds, and whether the call serves it (else its rows are left unwritten).
-__device__ __forceinline__ void load_bounds(const PagedParams &p, PagedTile &t) {
-    t.start = uniform(p.cu[t.seq]);
-    const int L = uniform(p.cu[t.seq + 1]) - t.start;
-    t.lk = uniform(p.lens[t.seq]);
-    t.off = t.lk - L;
-    t.rows = L * p.group;
-    t.valid = L > 0 && L <= p.max_seqlen && t.lk >= 0 && t.lk <= p.max_seqlen_k &&
-              t.lk <= (int64_t)p.max_pages * p.page && t.start >= 0 && (int64_t)t.start + L <= p.total_q;
-}
-
-// Tile `entry` of the call. Every wave finds it from the bounds: 64 sequences at a time, one per lane,
-// their tiles numbered by a scan.
-__device__ __forceinline__ PagedTile find_tile(const PagedParams &p, int entry, int bm) {
-    PagedTile t;
-    t.valid = false;
-    t.seq = entry;
-    t.row0 = 0;
-    if (!p.one_tile) {
-        const int lane = threadIdx.x & 63;
-        for (int base = 0;; base += 64) {
-            if (base >= p.n_seq) return t;
-            const int s = base + lane;
-            int n = 0;
-            if (s < p.n_seq) {
-                const int L = p.cu[s + 1] - p.cu[s];
-                if (L > 0 && L <= p.max_seqlen) n = (int)(((int64_t)L * p.group + bm - 1) / bm);
-            }
-            const int upto = wave_scan(n), all = __builtin_amdgcn_readlane(upto, 63);
-            if (entry < all) {
-                const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > entry));
-                t.seq = base + who;
-                t.row0 = (entry - __builtin_amdgcn_readlane(upto - n, who)) * bm;
-                break;
-            }
-            entry -= all;
-        }
+__device__ __forceinline__ Lanes lanes_from(const PagedParams &p, int base) {
+    Lanes q;
+    q.start = q.rows = q.lk = 0;
+    const int s = base + (int)(threadIdx.x & 63);
+    if (s < p.n_seq) {
+        q.start = p.cu[s];
+        const int L = p.cu[s + 1] - q.start;
+        q.lk = p.lens[s];
+        if (L > 0 && L <= p.max_seqlen && q.lk >= 0 && q.lk <= p.max_seqlen_k && q.lk <= (int64_t)p.max_pages * p.page &&
+            q.start >= 0 && (int64_t)q.start + L <= p.total_q)
+            q.rows = L * p.group;
     }
-    load_bounds(p, t);
-    t.valid = t.valid && t.row0 < t.rows;
-    return t;
+    return q;
 }
 
-// Keys [klo, khi) that some of the tile's rows reach by position, klo on a multiple of 64.
-__device__ __forceinline__ void tile_keys(const PagedParams &p, const PagedTile &t, int bm, int &klo, int &khi) {
-    const int t0 = t.row0 / p.group, t1 = (min(t.rows, t.row0 + bm) - 1) / p.group;
-    klo = p.wl >= 0 ? max(0, t.off + t0 - p.wl) & ~63 : 0;
-    khi = t.lk;
-    if (p.wr >= 0) khi = (int)max((int64_t)0, min((int64_t)t.lk, (int64_t)t.off + t1 + 1 + p.wr));
-}
-
-__device__ __forceinline__ int tile_chunks(const PagedParams &p, int klo, int khi) {
-    return max(1, (khi - klo + p.chunk - 1) / p.chunk);
+// Keys [klo, khi) that some of the rows [row0, row1) of a sequence reach by position, klo on a multiple of 64.
+// `off` is the key position of its first new token.
+__device__ __forceinline__ void keys_of(const PagedParams &p, int off, int lk, int row0, int row1, int &klo, int &khi) {
+    klo = p.wl >= 0 ? max(0, off + row0 / p.group - p.wl) & ~63 : 0;
+    khi = lk;
+    if (p.wr >= 0) khi = (int)max((int64_t)0, min((int64_t)lk, (int64_t)off + (row1 - 1) / p.group + 1 + p.wr));
 }
 
 // A masked key may hold an infinity or NaN, whose product with a zero probability is NaN. In blocks that
@@ -137,37 +107,121 @@ __device__ __forceinline__ bool reaches(const PagedParams &p, int pos, int key, 
     return key < khi && (p.wl < 0 || pos - key <= p.wl) && (p.wr < 0 || key - pos <= p.wr);
 }
 
-// Place of a row's share of one chunk, to be added to the other chunks' by paged_merge_kernel.
-__device__ __forceinline__ int64_t paged_slot(const PagedParams &p, int chunk, int row, int head) {
-    return ((int64_t)chunk * p.total_q + row) * p.hq + head;
-}
-
 // The 16 keys from `key` on (a multiple of 16) lie in a mapped page.
 __device__ __forceinline__ bool mapped16(const PagedParams &p, PageIds table, int key) {
     return (uint32_t)table[min(page_of(p, key), p.max_pages - 1)] < (uint32_t)p.n_pages;
 }
 
-// Tiles of 128 rows, four waves of 32, over keys that all of them read from LDS: chunks of prompts,
-// and any call. Two stages of 64 keys (32 at head_dim 256), filled by direct global-to-LDS loads of the
-// next while the waves work on one: 64 KB, two workgroups per CU (head_dim 64: three stages, 48 KB).
+// ----------------------------------------------------------------------------- many rows
+
+// Items of paged_tile_kernel: a query tile of 128 rows over a chunk of its keys. The chunk is as long as brings
+// the call to about `goal` workgroups: few tiles are split until they fill the chip, many stay whole, and
+// sequences of any lengths are cut alike. Every wave works this out from the bounds, 64 sequences at a time.
+constexpr int kTileRows = 128;
+constexpr int kChunkSteps = 4;  // of 64 keys, at least
+
+struct TileLanes {
+    Lanes seq;
+    int tiles, reach;  // query tiles, and the most steps of 64 keys that one reaches
+};
+
+__device__ __forceinline__ TileLanes tile_lanes(const PagedParams &p, int base) {
+    TileLanes t;
+    t.seq = lanes_from(p, base);
+    t.tiles = t.seq.rows > p.few ? (t.seq.rows + kTileRows - 1) / kTileRows : 0;
+    int64_t keys = t.seq.lk;
+    if (p.wl >= 0 && p.wr >= 0) keys = min(keys, (int64_t)p.wl + p.wr + (kTileRows - 1) / p.group + 2 + 64);
+    t.reach = (int)((keys + 63) >> 6);
+    return t;
+}
+
+// Steps of a chunk (SPLIT calls).
+__device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes &first) {
+    uint64_t sum = (uint64_t)first.tiles * first.reach;
+    for (int base = 64; base < p.n_seq; base += 64) {
+        const TileLanes t = tile_lanes(p, base);
+        sum += (uint64_t)t.tiles * t.reach;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((unsigned long long)sum, d);
+    const uint64_t steps = (sum * p.hkv + p.goal - 1) / p.goal;
+    return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 25)));
+}
+
+// The chunks of a sequence's tiles, at most; and its items that leave parts, one for each chunk of a tile.
+__device__ __forceinline__ int chunks_of(const TileLanes &t, int steps) { return max(1, (t.reach + steps - 1) / steps); }
+__device__ __forceinline__ int split_items(const TileLanes &t, int steps) {
+    const int n = chunks_of(t, steps);
+    return n > 1 ? t.tiles * n : 0;
+}
+
+struct TileItem {
+    int seq, start, rows, lk, off, row0, chunk;
+    int slot;   // the item's place among those that leave parts
+    bool valid;
+};
+
+template <bool SPLIT>
+__device__ __forceinline__ TileItem find_item(const PagedParams &p, int entry, int &steps) {
+    TileItem it;
+    it.valid = false;
+    TileLanes t = tile_lanes(p, 0);
+    if constexpr (SPLIT) steps = chunk_steps(p, t);
+    for (int base = 0, slots = 0;;) {
+        const int n = SPLIT ? t.tiles * chunks_of(t, steps) : t.tiles;
+        const int upto = wave_scan(n), all = __builtin_amdgcn_readlane(upto, 63);
+        int parts = 0;
+        if constexpr (SPLIT) parts = wave_scan(split_items(t, steps));
+        if (entry < all) {
+            const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > entry));
+            const int at = entry - __builtin_amdgcn_readlane(upto - n, who), tiles = __builtin_amdgcn_readlane(t.tiles, who);
+            it.seq = base + who;
+            it.start = __builtin_amdgcn_readlane(t.seq.start, who);
+            it.rows = __builtin_amdgcn_readlane(t.seq.rows, who);
+            it.lk = __builtin_amdgcn_readlane(t.seq.lk, who);
+            it.off = it.lk - it.rows / p.group;
+            it.chunk = SPLIT ? at / tiles : 0;  // a chunk's tiles side by side: they read the same keys
+            it.row0 = (at - it.chunk * tiles) * kTileRows;
+            if constexpr (SPLIT)
+                it.slot = slots + __builtin_amdgcn_readlane(parts - split_items(t, steps), who) + at;
+            it.valid = true;
+            return it;
+        }
+        entry -= all;
+        base += 64;
+        if (base >= p.n_seq) return it;
+        if constexpr (SPLIT) slots += __builtin_amdgcn_readlane(parts, 63);
+        t = tile_lanes(p, base);
+    }
+}
+
+// First slot of an item's rows, row r of the tile at slot + r.
+__device__ __forceinline__ int64_t tile_slot(const PagedParams &p, int item, int kvh) {
+    return p.tile_slots + ((int64_t)item * p.hkv + kvh) * kTileRows;
+}
+
+// Four waves of 32 rows over keys that all of them read from LDS: chunks of prompts, and any call. Two stages
+// of 64 keys (32 at head_dim 256), filled by direct global-to-LDS loads of the next while the waves work on
+// one: 64 KB, two workgroups per CU (head_dim 64: three stages, 48 KB).
 template <int D, bool SPLIT>
 __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
-    constexpr int BM = 128, BN = D == 256 ? 32 : 64, NS = D == 64 ? 3 : 2;
+    constexpr int BM = kTileRows, BN = D == 256 ? 32 : 64, NS = D == 64 ? 3 : 2;
     constexpr int NB = BN / 32, DC = D / 16, DB = D / 32, CPR = D / 8;
     constexpr int TILE = BN * D, UPW = TILE / 8 / 64 / 4, LPS = 2 * UPW, KPW = BN / 4;
     static_assert(UPW == 2 || UPW == 4, "loads go out four at a time");
     __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
 
     const int entry = blockIdx.x / p.hkv, kvh = blockIdx.x - entry * p.hkv;
-    const PagedTile t = find_tile(p, entry, BM);
+    int steps = 0;
+    const TileItem t = find_item<SPLIT>(p, entry, steps);
     if (!t.valid) return;
     int klo, khi;
-    tile_keys(p, t, BM, klo, khi);
-    const int chunks = SPLIT ? tile_chunks(p, klo, khi) : 1;
+    keys_of(p, t.off, t.lk, t.row0, min(t.rows, t.row0 + BM), klo, khi);
+    const bool split = SPLIT && khi - klo > 64 * steps;
     if constexpr (SPLIT) {
-        if ((int)blockIdx.y >= chunks) return;
-        klo += blockIdx.y * p.chunk;
-        khi = min(khi, klo + p.chunk);
+        if (t.chunk > 0 && khi - klo <= 64 * t.chunk * steps) return;  // the tile reaches less than others
+        klo += 64 * t.chunk * steps;
+        khi = min(khi, klo + 64 * steps);
     }
     const int ntiles = khi > klo ? (khi - klo + BN - 1) / BN : 0;
 
@@ -354,9 +408,9 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
     if (!wave_active) return;
     const float lsum = (ls[0] + ls[1]) + (ls[2] + ls[3]);
     const float l = lsum + __shfl_xor(lsum, 32);
-    if (SPLIT && chunks > 1) {
+    if (split) {
         if (row >= t.rows) return;
-        const int64_t slot = paged_slot(p, blockIdx.y, t.start + token, head);
+        const int64_t slot = tile_slot(p, t.slot, kvh) + 32 * wave + col;
         float *dst = p.part_o + slot * D + 4 * kg;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -378,43 +432,70 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
     store_block<DB, false>(o, inv, kg, o_rs, ooff, o_rs, 0);
 }
 
-// Tiles of 16 NR rows: single decoded tokens, a few drafted ones. There is one row tile per (sequence, kv
-// head) or little more, and the time is that of reading its keys once, so the waves share nothing: each takes
-// every NW-th 32-key step of the workgroup's chunk through stages of its own (no barrier; a step waits for the
-// wave's own loads), and the waves' sums are added at the end. Products on v_mfma_f32_16x16x32_bf16, lane l:
-// c16 = l % 16, g4 = l / 16:
+// ----------------------------------------------------------------------------- few rows
+
+// Calls of at most 32 rows per sequence and kv head (single decoded tokens, a few drafted ones) last as long as
+// reading their keys once, if all waves read to the end. The keys of one kv head, all sequences in a row, are
+// cut into steps of 32 and dealt in equal runs to the head's waves: a run may end one sequence and begin the
+// next, so lengths however unequal leave no wave idle, and a wave begins at most one or two sequences. (Equal
+// chunks of each sequence, two waves each: 64 sequences of U{512..8192} keys left 10 % to the last to end.)
+constexpr int kRunSteps = 2;  // at least, per wave
+
+struct RowLanes {
+    Lanes seq;
+    int base, n, upto, all;  // steps, their inclusive sum over the lanes, their total
+};
+
+__device__ __forceinline__ RowLanes row_lanes(const PagedParams &p, int base) {
+    RowLanes r;
+    r.base = base;
+    r.seq = lanes_from(p, base);
+    r.n = 0;
+    if (r.seq.rows > 0 && r.seq.rows <= p.few) {
+        int klo, khi;
+        keys_of(p, r.seq.lk - r.seq.rows / p.group, r.seq.lk, 0, r.seq.rows, klo, khi);
+        r.n = max(1, (khi - klo + 31) >> 5);  // a sequence without a key in reach still has rows to write
+    }
+    r.upto = wave_scan(r.n);
+    r.all = __builtin_amdgcn_readlane(r.upto, 63);
+    return r;
+}
+
+// Steps of a wave's run: all sequences' steps over the head's waves.
+__device__ __forceinline__ int row_run(const PagedParams &p, int total) {
+    return max(kRunSteps, (total + p.workers - 1) / p.workers);
+}
+
+// Place of a part: a wave writes at most two, of the sequence that began before its run and of the one
+// that goes on past it.
+__device__ __forceinline__ int64_t row_slot(const PagedParams &p, int wave, int which) {
+    return ((int64_t)wave * 2 + which) * p.few;
+}
+
+// One wave, with LDS stages of its own: no barrier, a step waits for the wave's own loads. Products on
+// v_mfma_f32_16x16x32_bf16, lane l: c16 = l % 16, g4 = l / 16:
 //  * S^T = K . Q^T per 16 keys: A = key c16 by dims 32 c + 8 g4 .., B = the lane's row; lane l then holds, for
 //    row c16, keys 4 g4 + i.
 //  * O^T = V^T . P^T per 16 dims: B = the lane's own 8 probabilities, k-slot 8 g4 + i standing for key
 //    4 g4 + i and 8 g4 + 4 + i for key 16 + 4 g4 + i; A = V^T for the same keys by two transposing reads;
 //    lane l accumulates dims 16 db + 4 g4 + i of row c16.
-template <int D, int NR, int NW, int NS, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void paged_row_kernel(PagedParams p) {
-    constexpr int BM = 16 * NR, BN = 32, DC = D / 32, DB = D / 16, CPR = D / 8;
-    constexpr int TILE = BN * D;           // elements of a step's K (or V)
-    constexpr int LH = CPR / 4;            // 1 KB loads of 16 keys
-    constexpr int LPS = 4 * LH;            // loads of a step
+template <int D, int NR, int NS>
+__global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
+    constexpr int BN = 32, DC = D / 32, DB = D / 16, CPR = D / 8;
+    constexpr int TILE = BN * D;  // elements of a step's K (or V)
+    constexpr int LH = CPR / 4;   // 1 KB loads of 16 keys
+    constexpr int LPS = 4 * LH;   // loads of a step
     static_assert(LH == 2 || LH % 4 == 0, "loads go out four at a time");
-    __shared__ __attribute__((aligned(16))) __bf16 ring[NW][NS][2][TILE];
-    static_assert(sizeof(ring) >= (size_t)NW * BM * D * 4, "the waves' sums fit the ring");
-    __shared__ float stat[NW][2][BM];
+    __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
 
-    const int entry = blockIdx.x / p.hkv, kvh = blockIdx.x - entry * p.hkv;
-    const PagedTile t = find_tile(p, entry, BM);
-    if (!t.valid) return;
-    int klo, khi;
-    tile_keys(p, t, BM, klo, khi);
-    const int chunks = SPLIT ? tile_chunks(p, klo, khi) : 1;
-    if constexpr (SPLIT) {
-        if ((int)blockIdx.y >= chunks) return;
-        klo += blockIdx.y * p.chunk;
-        khi = min(khi, klo + p.chunk);
-    }
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int c16 = lane & 15, g4 = lane >> 4;
-    const int all = khi > klo ? (khi - klo + BN - 1) / BN : 0;       // steps of the workgroup
-    const int steps = all > wave ? (all - wave + NW - 1) / NW : 0;  // and of the wave
-    const PageIds table = page_ids_of(p, t.seq);
+    const int kvh = blockIdx.x % p.hkv, worker = blockIdx.x / p.hkv;
+    const int lane = threadIdx.x, c16 = lane & 15, g4 = lane >> 4;
+    RowLanes seqs = row_lanes(p, 0);
+    int total = seqs.all;
+    for (int base = 64; base < p.n_seq; base += 64) total += row_lanes(p, base).all;
+    const int run = row_run(p, total), first = worker * run;
+    if (first >= total) return;
+    const int last = min(total, first + run);
 
     const int k_row = (int)p.k_st * 2, v_row = (int)p.v_st * 2;
     int koff[LH], voff[LH];
@@ -424,308 +505,415 @@ __global__ __launch_bounds__(64 * NW) void paged_row_kernel(PagedParams p) {
         koff[j] = key * k_row + ch * 16;
         voff[j] = key * v_row + ch * 16;
     }
-    const uint32_t ring_base = uniform((int)lds_addr(&ring[wave][0][0][0]));
-    auto key_of = [&](int step) { return klo + (step * NW + wave) * BN; };
-    // The ids of the pages that hold a step's two halves.
-    auto page_ids = [&](int step) {
-        const int key = key_of(step), last = p.max_pages - 1;
-        return int2{table[min(page_of(p, key), last)], table[min(page_of(p, key + 16), last)]};
-    };
-    auto mapped = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
-    auto issue = [&](int stage, int step, int2 ids) {
-        const uint32_t base = ring_base + stage * (4 * TILE);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int key0 = key_of(step) + 16 * h, slot = key0 - page_of(p, key0) * p.page, id = h ? ids.y : ids.x;
-            const int rows = mapped(id) ? max(0, min(p.page - slot, t.lk - key0)) : 0;
-            const int64_t page = mapped(id) ? id : 0;
-            const __amdgpu_buffer_rsrc_t k_rs =
-                make_rsrc(p.k + page * p.k_sp + slot * p.k_st + kvh * p.k_sh, rows_bytes(rows, p.k_st, D));
-            const __amdgpu_buffer_rsrc_t v_rs =
-                make_rsrc(p.v + page * p.v_sp + slot * p.v_st + kvh * p.v_sh, rows_bytes(rows, p.v_st, D));
-            const uint32_t kb = base + h * LH * 1024, vb = kb + 2 * TILE;
-            if constexpr (LH == 2) {
-                const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
-                const int o4[4] = {koff[0], koff[1], voff[0], voff[1]};
-                dma16x4(l4, o4, k_rs, v_rs);
-            } else {
-#pragma unroll
-                for (int j = 0; j < LH; j += 4) {
-                    const uint32_t lk[4] = {kb + j * 1024, kb + j * 1024 + 1024, kb + j * 1024 + 2048, kb + j * 1024 + 3072};
-                    const int ok[4] = {koff[j], koff[j + 1], koff[j + 2], koff[j + 3]};
-                    dma16x4(lk, ok, k_rs, k_rs);
-                }
-#pragma unroll
-                for (int j = 0; j < LH; j += 4) {
-                    const uint32_t lv[4] = {vb + j * 1024, vb + j * 1024 + 1024, vb + j * 1024 + 2048, vb + j * 1024 + 3072};
-                    const int ov[4] = {voff[j], voff[j + 1], voff[j + 2], voff[j + 3]};
-                    dma16x4(lv, ov, v_rs, v_rs);
-                }
-            }
-        }
-    };
-
-    // Query fragments: lane (c16, g4) holds dims 32 c + 8 g4 .. of row c16 of each block.
-    int pos[NR];
-    bf16x8 qf[NR][DC];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        const int row = t.row0 + 16 * r + c16, token = row / p.group, head = kvh * p.group + row - token * p.group;
-        pos[r] = t.off + token;
-        const __bf16 *src = p.q + (int64_t)(t.start + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g4;
-#pragma unroll
-        for (int c = 0; c < DC; ++c) qf[r][c] = row < t.rows ? ld_g16(src + 32 * c) : bf16x8{};
-    }
-    // Key positions of the tile's first row and past its last.
-    const int p0 = t.off + t.row0 / p.group, p1 = t.off + (min(t.rows, t.row0 + BM) - 1) / p.group + 1;
     // Place of the operands' first chunk in a stage; the swizzle exchanges whole units and depends on the
     // key's low four bits alone, so chunk c is 32 c elements on by exclusive or, and 16 keys on by sum.
     const int vkey = 4 * g4 + (c16 >> 2), vdim = 4 * (c16 & 3);
     const int kbase = c16 * D + (g4 ^ swz<CPR>(c16)) * 8;
     const int vbase = vkey * D + ((vdim >> 3) ^ swz<CPR>(vkey)) * 8 + (vdim & 4);
-
-    f32x4 o[NR][DB];
-    float m[NR], ls[NR];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[r][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m[r] = kNegInf;
-        ls[r] = 0.0f;
-    }
+    const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
     const float c2 = p.c;
 
-    int2 held[NS];  // page ids of the steps in the ring, and of the next to issue
-    if (steps > 0) {
+    int before = 0;  // steps of the sequences before seqs.base
+    for (int x = first; x < last;) {
+        while (before + seqs.all <= x) {
+            before += seqs.all;
+            seqs = row_lanes(p, seqs.base + 64);
+        }
+        const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + seqs.upto > x));
+        const int begin = before + __builtin_amdgcn_readlane(seqs.upto - seqs.n, who);
+        const int end = before + __builtin_amdgcn_readlane(seqs.upto, who);
+        const int start = __builtin_amdgcn_readlane(seqs.seq.start, who), nrows = __builtin_amdgcn_readlane(seqs.seq.rows, who);
+        const int lk = __builtin_amdgcn_readlane(seqs.seq.lk, who), off = lk - nrows / p.group;
+        int klo, khi;
+        keys_of(p, off, lk, 0, nrows, klo, khi);
+        const int key_first = klo + 32 * (x - begin), steps = min(last, end) - x;
+        const bool whole_row = begin >= first && end <= last;  // no other wave has keys of these rows
+        const int slot_of = begin < first ? 0 : 1;
+        x += steps;
+
+        const PageIds table = page_ids_of(p, seqs.base + who);
+        // The ids of the pages that hold a step's two halves.
+        auto page_ids = [&](int step) {
+            const int key = key_first + 32 * step, top = p.max_pages - 1;
+            if (top < 0) return int2{-1, -1};
+            return int2{table[min(page_of(p, key), top)], table[min(page_of(p, key + 16), top)]};
+        };
+        auto mapped = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
+        auto issue = [&](int stage, int step, int2 ids) {
+            const uint32_t base = ring_base + stage * (4 * TILE);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key0 = key_first + 32 * step + 16 * h, slot = key0 - page_of(p, key0) * p.page;
+                const int id = h ? ids.y : ids.x;
+                const int rows = mapped(id) ? max(0, min(p.page - slot, lk - key0)) : 0;
+                const int64_t page = mapped(id) ? id : 0;
+                const __amdgpu_buffer_rsrc_t k_rs =
+                    make_rsrc(p.k + page * p.k_sp + slot * p.k_st + kvh * p.k_sh, rows_bytes(rows, p.k_st, D));
+                const __amdgpu_buffer_rsrc_t v_rs =
+                    make_rsrc(p.v + page * p.v_sp + slot * p.v_st + kvh * p.v_sh, rows_bytes(rows, p.v_st, D));
+                const uint32_t kb = base + h * LH * 1024, vb = kb + 2 * TILE;
+                if constexpr (LH == 2) {
+                    const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
+                    const int o4[4] = {koff[0], koff[1], voff[0], voff[1]};
+                    dma16x4(l4, o4, k_rs, v_rs);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < LH; j += 4) {
+                        const uint32_t l = kb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
+                        const int o4[4] = {koff[j], koff[j + 1], koff[j + 2], koff[j + 3]};
+                        dma16x4(l4, o4, k_rs, k_rs);
+                    }
+#pragma unroll
+                    for (int j = 0; j < LH; j += 4) {
+                        const uint32_t l = vb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
+                        const int o4[4] = {voff[j], voff[j + 1], voff[j + 2], voff[j + 3]};
+                        dma16x4(l4, o4, v_rs, v_rs);
+                    }
+                }
+            }
+        };
+
+        // Query fragments: lane (c16, g4) holds dims 32 c + 8 g4 .. of row c16 of each block.
+        int pos[NR];
+        bf16x8 qf[NR][DC];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = 16 * r + c16, token = row / p.group, head = kvh * p.group + row - token * p.group;
+            pos[r] = off + token;
+            const __bf16 *src = p.q + (int64_t)(start + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g4;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) qf[r][c] = row < nrows ? ld_g16(src + 32 * c) : bf16x8{};
+        }
+        const int p0 = off, p1 = off + (nrows - 1) / p.group + 1;  // key positions of the first row, past the last
+
+        f32x4 o[NR][DB];
+        float m[NR], ls[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[r][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m[r] = kNegInf;
+            ls[r] = 0.0f;
+        }
+        int2 held[NS];  // page ids of the steps in the ring, and of the next to issue
 #pragma unroll
         for (int s = 0; s < NS; ++s) held[s] = page_ids(s);
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the sequence before has read its stages
 #pragma unroll
         for (int s = 0; s < NS - 1; ++s)
             if (s < steps) issue(s, s, held[s]);
-    }
-    // The query rows' wait, here once: at their first use it would stand in the loop, and wait for the
-    // loads ahead in every step.
+        // The query rows' wait, here once: at their first use it would stand in the loop, and wait for the
+        // loads ahead in every step.
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[r][c]));
-    for (int step = 0; step < steps; ++step) {
-        // The stage of the step before is free once its reads are done; a step's loads are complete once at
-        // most the later steps' are in flight.
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-        const int stage = step % NS, ahead = step + NS - 1;
-        if (ahead < steps) issue(ahead % NS, ahead, held[NS - 1]);
-        const int later = min(steps, ahead + 1) - step - 1;
-        if (NS >= 3 && later >= 2) wait_vmcnt<2 * LPS>();
-        else if (later >= 1) wait_vmcnt<LPS>();
-        else wait_vmcnt<0>();
-        const int2 ids = held[0];
+            for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[r][c]));
+        for (int step = 0; step < steps; ++step) {
+            // The stage of the step before is free once its reads are done; a step's loads are complete once at
+            // most the later steps' are in flight.
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+            const int stage = step % NS, ahead = step + NS - 1;
+            if (ahead < steps) issue(ahead % NS, ahead, held[NS - 1]);
+            const int later = min(steps, ahead + 1) - step - 1;
+            if (NS >= 4 && later >= 3) wait_vmcnt<NS >= 4 ? 3 * LPS : 0>();
+            else if (NS >= 3 && later >= 2) wait_vmcnt<2 * LPS>();
+            else if (later >= 1) wait_vmcnt<LPS>();
+            else wait_vmcnt<0>();
+            const int2 ids = held[0];
 #pragma unroll
-        for (int s = 0; s < NS - 1; ++s) held[s] = held[s + 1];
-        held[NS - 1] = page_ids(step + NS);
-        const __bf16 *kt = &ring[wave][stage][0][0], *vt = &ring[wave][stage][1][0];
-        const int kt0 = key_of(step);
-        const bool gap = !mapped(ids.x) || !mapped(ids.y);
-        const bool whole = !gap && block_full(kt0, khi, p0, p1, p.wl, p.wr);
-        f32x4 sc[NR][2];
+            for (int s = 0; s < NS - 1; ++s) held[s] = held[s + 1];
+            held[NS - 1] = page_ids(step + NS);
+            const __bf16 *kt = &ring[stage][0][0], *vt = &ring[stage][1][0];
+            const int kt0 = key_first + 32 * step;
+            const bool whole = mapped(ids.x) && mapped(ids.y) && block_full(kt0, khi, p0, p1, p.wl, p.wr);
+            f32x4 sc[NR][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 2; ++b) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) sc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = 0; r < NR; ++r) sc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int c = 0; c < DC; ++c) {
-                const bf16x8 ka = ld_s16(kt + 16 * b * D + (kbase ^ (32 * c)));
+                for (int c = 0; c < DC; ++c) {
+                    const bf16x8 ka = ld_s16(kt + 16 * b * D + (kbase ^ (32 * c)));
 #pragma unroll
-                for (int r = 0; r < NR; ++r)
-                    sc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[r][c], sc[r][b], 0, 0, 0);
+                    for (int r = 0; r < NR; ++r)
+                        sc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[r][c], sc[r][b], 0, 0, 0);
+                }
             }
-        }
-        bf16x8 pb[NR];
+            bf16x8 pb[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            if (!whole) {
-                uint32_t km = key_mask(kt0, g4, pos[r], khi, p.wl, p.wr);  // bit x: key kt0 + 4 g4 + x
-                const uint32_t low = (1u << (16 - 4 * g4)) - 1u;
-                km &= (mapped(ids.x) ? low : 0u) | (mapped(ids.y) ? ~low : 0u);
+            for (int r = 0; r < NR; ++r) {
+                if (!whole) {
+                    uint32_t km = key_mask(kt0, g4, pos[r], khi, p.wl, p.wr);  // bit x: key kt0 + 4 g4 + x
+                    const uint32_t low = (1u << (16 - 4 * g4)) - 1u;          // of the step's first 16 keys
+                    km &= (mapped(ids.x) ? low : 0u) | (mapped(ids.y) ? ~low : 0u);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[r][b][i] = mask_score(sc[r][b][i], km, 16 * b + i);
+                        for (int i = 0; i < 4; ++i) sc[r][b][i] = mask_score(sc[r][b][i], km, 16 * b + i);
+                }
+                const f32x4 &a = sc[r][0], &z = sc[r][1];
+                const float mx =
+                    fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+                // Raised only when a row exceeds it by 2^8; the four lanes of a row share m.
+                if (wave_any(mx * c2 > m[r] + 8.0f)) {
+                    float top = fmaxf(mx, __shfl_xor(mx, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float mnew = fmaxf(m[r], top * c2);
+                    const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m[r] - mnew);
+                    m[r] = mnew;
+                    ls[r] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) o[r][db] *= alpha;
+                }
+                const float muse = m[r] == kNegInf ? 0.0f : m[r];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pb[r][i] = (__bf16)exp2_fast(fmaf(sc[r][i >> 2][i & 3], c2, -muse));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ls[r] = sum2(pb[r], i, ls[r]);
             }
-            const f32x4 &a = sc[r][0], &z = sc[r][1];
-            const float mx = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
-            // Raised only when a row exceeds it by 2^8; the four lanes of a row share m.
-            if (wave_any(mx * c2 > m[r] + 8.0f)) {
-                float top = fmaxf(mx, __shfl_xor(mx, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float mnew = fmaxf(m[r], top * c2);
-                const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m[r] - mnew);
-                m[r] = mnew;
-                ls[r] *= alpha;
+            auto values = [&](int db) {
+                const __bf16 *at = vt + (vbase ^ (16 * db));
+                const bf16x4 lo = tr16(at), hi = tr16(at + 16 * D);
+                return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            uint32_t bad = 0;
 #pragma unroll
-                for (int db = 0; db < DB; ++db) o[r][db] *= alpha;
+            for (int db = 0; db < DB; ++db) {
+                bf16x8 va = values(db);
+                if (!whole) bad |= clean8(va);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) o[r][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[r], o[r][db], 0, 0, 0);
             }
-            const float muse = m[r] == kNegInf ? 0.0f : m[r];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pb[r][i] = (__bf16)exp2_fast(fmaf(sc[r][i >> 2][i & 3], c2, -muse));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ls[r] = sum2(pb[r], i, ls[r]);
-        }
-        auto values = [&](int db) {
-            const __bf16 *at = vt + (vbase ^ (16 * db));
-            const bf16x4 lo = tr16(at), hi = tr16(at + 16 * D);
-            return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
-        uint32_t bad = 0;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            bf16x8 va = values(db);
-            if (!whole) bad |= clean8(va);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) o[r][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[r], o[r][db], 0, 0, 0);
-        }
-        if (wave_any(bad != 0)) {
+            if (wave_any(bad != 0)) {
 #pragma unroll 1
-            for (int key = 0; key < BN; ++key) {
+                for (int key = 0; key < BN; ++key) {
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {  // dims 16 db + 4 g4 ..
-                    const int unit = (2 * db + (g4 >> 1)) ^ swz<CPR>(key);
-                    const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vt + key * D + unit * 8 + 4 * (g4 & 1));
+                    for (int db = 0; db < DB; ++db) {  // dims 16 db + 4 g4 ..
+                        const int unit = (2 * db + (g4 >> 1)) ^ swz<CPR>(key);
+                        const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vt + key * D + unit * 8 + 4 * (g4 & 1));
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const bool reach = reaches(p, pos[r], kt0 + key, khi);
+                        for (int r = 0; r < NR; ++r) {
+                            const bool reach = reaches(p, pos[r], kt0 + key, khi);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[r][db][i] += reach ? only_nonfinite(v4[i]) : 0.0f;
+                            for (int i = 0; i < 4; ++i) o[r][db][i] += reach ? only_nonfinite(v4[i]) : 0.0f;
+                        }
                     }
                 }
             }
         }
-    }
-
-    // The waves' sums through LDS, then one thread per four dims of a row weighs and adds them.
-    __syncthreads();
-    float *sums = reinterpret_cast<float *>(&ring[0][0][0][0]);  // [NW][BM][D]
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        float l = ls[r] + __shfl_xor(ls[r], 16);
-        l += __shfl_xor(l, 32);
-        if (g4 == 0) {
-            stat[wave][0][16 * r + c16] = m[r];
-            stat[wave][1][16 * r + c16] = l;
-        }
+        for (int r = 0; r < NR; ++r) {
+            float l = ls[r] + __shfl_xor(ls[r], 16);
+            l += __shfl_xor(l, 32);
+            const int row = 16 * r + c16;
+            if (row >= nrows) continue;
+            if (whole_row) {
+                const int token = row / p.group, head = kvh * p.group + row - token * p.group;
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+                __bf16 *dst = p.o + (int64_t)(start + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g4;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-            *reinterpret_cast<f32x4 *>(sums + (wave * BM + 16 * r + c16) * D + 16 * db + 4 * g4) = o[r][db];
-    }
-    __syncthreads();
-    const int rows = min(BM, t.rows - t.row0);
-    for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
-        const int r = i / (D / 4), dim = 4 * (i - r * (D / 4));
-        float mx = stat[0][0][r];
+                for (int db = 0; db < DB; ++db)
+                    *reinterpret_cast<bf16x4 *>(dst + 16 * db) = round4<false>(
+                        o[r][db][0] * inv, o[r][db][1] * inv, o[r][db][2] * inv, o[r][db][3] * inv, bf16x4{});
+            } else {
+                const int64_t slot = row_slot(p, blockIdx.x, slot_of) + row;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) mx = fmaxf(mx, stat[w][0][r]);
-        float l = 0.0f;
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float weight = stat[w][0][r] == kNegInf ? 0.0f : exp2_fast(stat[w][0][r] - mx);
-            l = fmaf(stat[w][1][r], weight, l);
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(sums + (w * BM + r) * D + dim);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = fmaf(y[j], weight, x[j]);
-        }
-        const int row = t.row0 + r, token = row / p.group, head = kvh * p.group + row - token * p.group;
-        if (SPLIT && chunks > 1) {
-            const int64_t slot = paged_slot(p, blockIdx.y, t.start + token, head);
-            *reinterpret_cast<f32x4 *>(p.part_o + slot * D + dim) = x;
-            if (dim == 0) {
-                p.part_ml[2 * slot] = mx;
-                p.part_ml[2 * slot + 1] = l;
+                for (int db = 0; db < DB; ++db)
+                    *reinterpret_cast<f32x4 *>(p.part_o + slot * D + 16 * db + 4 * g4) = o[r][db];
+                if (g4 == 0) {
+                    p.part_ml[2 * slot] = m[r];
+                    p.part_ml[2 * slot + 1] = l;
+                }
             }
-        } else {
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            *reinterpret_cast<bf16x4 *>(p.o + (int64_t)(t.start + token) * p.o_st + (int64_t)head * p.o_sh + dim) =
-                round4<false>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv, bf16x4{});
         }
     }
 }
 
-// Adds the chunks of split rows: one workgroup per (query row, head). The chunks' maxima and sums (at
-// most kMaxChunks) are read at once and turned into weights in LDS; then groups of D / 4 lanes take the
-// chunks in turn and their sums are added in a fixed order, so the result does not depend on which
-// workgroup finished first.
-constexpr int kMaxChunks = 1024;
+// ----------------------------------------------------------------------------- the parts' sums
 
-template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int bm, int max_chunks) {
-    constexpr int LPR = D / 4, GROUPS = 256 / LPR;
-    __shared__ float weight[kMaxChunks];
-    __shared__ float red[2][4];
-    __shared__ __attribute__((aligned(16))) float sums[GROUPS][D];
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int row = blockIdx.x, qh = blockIdx.y;  // packed token, query head
-    PagedTile t;
-    t.seq = -1;
+// Adds the parts of split rows, weighed against the row's largest maximum, in a fixed order: the result does
+// not depend on which wave finished first. Rows of one part are already written.
+
+// Where a packed row of one query head has its parts: count (0 or 1: nothing to add), the first's slot, and the
+// others' base and step: part i > 0 is slot rest + i * step.
+struct RowParts {
+    int count;
+    int64_t first, rest, step;
+};
+
+// A packed row's sequence and where its parts lie, the same for all query heads. RUNS: sequences of few rows
+// have parts; TILES: the others have.
+struct RowPlace {
+    int token, rows, lk;                    // token < 0: a row that the call does not serve
+    int begin, end, run;                    // steps of its sequence, and of a wave's run
+    int item0, tiles, steps;                // its first item that leaves parts, its tiles, the steps of a chunk
+};
+
+template <bool RUNS, bool TILES>
+__device__ __forceinline__ RowPlace row_place(const PagedParams &p, int row) {
+    RowPlace r;
+    r.token = -1;
+    r.rows = r.lk = r.begin = r.end = r.item0 = r.tiles = r.steps = 0;
+    if constexpr (TILES) r.steps = chunk_steps(p, tile_lanes(p, 0));
+    int total = 0, items = 0;
     for (int base = 0; base < p.n_seq; base += 64) {
-        const int s = base + lane;
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(s < p.n_seq && p.cu[s] <= row && row < p.cu[s + 1]);
-        if (hit) {
-            t.seq = base + __builtin_ctzll(hit);
-            break;
+        const TileLanes t = tile_lanes(p, base);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(t.seq.rows > 0 && t.seq.start <= row &&
+                                                         row < t.seq.start + t.seq.rows / p.group);
+        const bool here = hit && r.token < 0;
+        const int who = here ? __builtin_ctzll(hit) : 0;
+        if (here) {
+            r.token = row - __builtin_amdgcn_readlane(t.seq.start, who);
+            r.rows = __builtin_amdgcn_readlane(t.seq.rows, who);
+            r.lk = __builtin_amdgcn_readlane(t.seq.lk, who);
+        }
+        if constexpr (RUNS) {
+            const RowLanes seqs = row_lanes(p, base);
+            if (here) {
+                r.begin = total + __builtin_amdgcn_readlane(seqs.upto - seqs.n, who);
+                r.end = total + __builtin_amdgcn_readlane(seqs.upto, who);
+            }
+            total += seqs.all;
+        }
+        if constexpr (TILES) {
+            const int n = split_items(t, r.steps), upto = wave_scan(n);
+            if (here) {
+                r.item0 = items + __builtin_amdgcn_readlane(upto - n, who);
+                r.tiles = __builtin_amdgcn_readlane(t.tiles, who);
+            }
+            items += __builtin_amdgcn_readlane(upto, 63);
+        } else if (!RUNS || (here && r.rows > p.few)) {
+            break;  // nothing more to know
         }
     }
-    if (t.seq < 0) return;
-    load_bounds(p, t);
-    if (!t.valid) return;
-    t.row0 = ((row - t.start) * p.group + qh % p.group) / bm * bm;
-    int klo, khi;
-    tile_keys(p, t, bm, klo, khi);
-    const int chunks = min(max_chunks, tile_chunks(p, klo, khi));
-    if (chunks <= 1) return;  // written by its one workgroup
-    const int64_t slot0 = paged_slot(p, 0, row, qh), stride = paged_slot(p, 1, 0, 0);
-    float2 ml[kMaxChunks / 256];
-    float mx = kNegInf;
-#pragma unroll
-    for (int i = 0; i < kMaxChunks / 256; ++i) {
-        ml[i] = float2{kNegInf, 0.0f};
-        if (tid + 256 * i < chunks) ml[i] = reinterpret_cast<const float2 *>(p.part_ml)[slot0 + (tid + 256 * i) * stride];
-        mx = fmaxf(mx, ml[i].x);
+    r.run = row_run(p, total);
+    return r;
+}
+
+template <bool RUNS, bool TILES>
+__device__ __forceinline__ RowParts parts_of(const PagedParams &p, const RowPlace &r, int qh) {
+    RowParts s;
+    s.count = 0;
+    s.first = s.rest = s.step = 0;
+    const int kvh = qh / p.group, at = r.token * p.group + qh - kvh * p.group;  // row of the sequence
+    if (r.token < 0) return s;
+    if (RUNS && r.rows <= p.few) {
+        const int w0 = r.begin / r.run;
+        s.count = (r.end - 1) / r.run - w0 + 1;
+        s.first = row_slot(p, w0 * p.hkv + kvh, 1) + at;
+        s.rest = row_slot(p, w0 * p.hkv + kvh, 0) + at;
+        s.step = row_slot(p, p.hkv, 0);
+    } else if (TILES && r.rows > p.few) {
+        const int tile = at / kTileRows;
+        int klo, khi;
+        keys_of(p, r.lk - r.rows / p.group, r.lk, tile * kTileRows, min(r.rows, (tile + 1) * kTileRows), klo, khi);
+        s.count = max(0, khi - klo + 64 * r.steps - 1) / (64 * r.steps);
+        s.first = s.rest = tile_slot(p, r.item0 + tile, kvh) + at - tile * kTileRows;
+        s.step = (int64_t)r.tiles * p.hkv * kTileRows;
     }
+    return s;
+}
+
+__device__ __forceinline__ int64_t part_at(const RowParts &r, int i) { return i == 0 ? r.first : r.rest + i * r.step; }
+
+__device__ __forceinline__ void store_merged(const PagedParams &p, int row, int qh, int dim, const f32x4 &o, float l) {
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    *reinterpret_cast<bf16x4 *>(p.o + (int64_t)row * p.o_st + (int64_t)qh * p.o_sh + dim) =
+        round4<false>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, bf16x4{});
+}
+
+// Many rows: a wave per row and 64 / (D / 4) query heads, D / 4 lanes each. No LDS and no barrier, so that the
+// chip's waves are on their loads (a workgroup per row and head: 2,048 rows of 12 heads of 64 in 6 parts
+// 47 us, this 16).
+template <int D, bool RUNS, bool TILES>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
+    constexpr int LPR = D / 4, HEADS = 64 / LPR, AHEAD = 4;
+    const int lane = threadIdx.x & 63, sub = lane % LPR, dim = 4 * sub, per = (p.hq + HEADS - 1) / HEADS;
+    const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+    if (item >= (int64_t)p.total_q * per) return;
+    const int row = (int)(item / per), qh = (int)(item - (int64_t)row * per) * HEADS + lane / LPR;
+    const RowPlace place = row_place<RUNS, TILES>(p, row);
+    RowParts parts = parts_of<RUNS, TILES>(p, place, min(qh, p.hq - 1));
+    if (qh >= p.hq) parts.count = 0;
+    if (!wave_any(parts.count > 1)) return;
+    const float2 *stats = reinterpret_cast<const float2 *>(p.part_ml);
+    float mx = kNegInf;
+    for (int i = sub; i < parts.count; i += LPR) mx = fmaxf(mx, stats[part_at(parts, i)].x);
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+    float l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = 0; wave_any(base < parts.count); base += LPR) {
+        const int n = min(LPR, parts.count - base);
+        const float2 ml = sub < n ? stats[part_at(parts, base + sub)] : float2{kNegInf, 0.0f};
+        const float w = ml.x == kNegInf ? 0.0f : exp2_fast(ml.x - mx);
+        l = fmaf(ml.y, w, l);
+        for (int c0 = 0; wave_any(c0 < n); c0 += AHEAD) {
+            f32x4 x[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (c0 + u < n) x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + part_at(parts, base + c0 + u) * D + dim);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const float wc = __shfl(w, ((lane / LPR) * LPR + c0 + u) & 63);  // every lane takes part
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = c0 + u < n ? fmaf(x[u][i], wc, o[i]) : o[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) l += __shfl_xor(l, d);
+    if (parts.count > 1) store_merged(p, row, qh, dim, o, l);
+}
+
+// Few rows, which may have many parts: 64 dims of a (row, query head) have a workgroup of their own, its
+// sixteen groups of lanes taking the parts in turn.
+constexpr int kMaxParts = 2048;
+
+template <int D, bool RUNS, bool TILES>
+__global__ __launch_bounds__(256) void paged_merge_long_kernel(PagedParams p) {
+    __shared__ float weight[kMaxParts];
+    __shared__ float red[2][4];
+    __shared__ __attribute__((aligned(16))) float sums[16][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int row = blockIdx.x, qh = blockIdx.y;
+    const RowParts parts = parts_of<RUNS, TILES>(p, row_place<RUNS, TILES>(p, row), qh);
+    const int count = min(parts.count, kMaxParts);
+    if (count <= 1) return;
+    const float2 *stats = reinterpret_cast<const float2 *>(p.part_ml);
+    float mx = kNegInf;
+    for (int i = tid; i < count; i += 256) mx = fmaxf(mx, weight[i] = stats[part_at(parts, i)].x);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
     if (lane == 0) red[0][wave] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     float l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMaxChunks / 256; ++i) {
-        const float w = ml[i].x == kNegInf ? 0.0f : exp2_fast(ml[i].x - mx);
-        weight[tid + 256 * i] = w;
-        l = fmaf(ml[i].y, w, l);
+    for (int i = tid; i < count; i += 256) {
+        const float w = weight[i] == kNegInf ? 0.0f : exp2_fast(weight[i] - mx);
+        weight[i] = w;
+        l = fmaf(stats[part_at(parts, i)].y, w, l);
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
     if (lane == 0) red[1][wave] = l;
     __syncthreads();
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const int g = tid / LPR, dim = 4 * (tid % LPR);
-    const float *src = p.part_o + slot0 * D + dim;
+    const int g = tid >> 4, at = 4 * (tid & 15), dim = 64 * blockIdx.z + at;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-    for (int c = g; c < chunks; c += GROUPS) {
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(src + c * stride * D);
+    for (int c = g; c < count; c += 16) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + part_at(parts, c) * D + dim);
         const float wc = weight[c];
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], wc, o[i]);
     }
-    *reinterpret_cast<f32x4 *>(&sums[g][dim]) = o;
+    *reinterpret_cast<f32x4 *>(&sums[g][at]) = o;
     __syncthreads();
     if (g != 0) return;
 #pragma unroll
-    for (int i = 1; i < GROUPS; ++i) o += *reinterpret_cast<const f32x4 *>(&sums[i][dim]);
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const bf16x4 y = round4<false>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, bf16x4{});
-    *reinterpret_cast<bf16x4 *>(p.o + (int64_t)row * p.o_st + (int64_t)qh * p.o_sh + dim) = y;
+    for (int i = 1; i < 16; ++i) o += *reinterpret_cast<const f32x4 *>(&sums[i][at]);
+    store_merged(p, row, qh, dim, o, l);
 }
 
 }  // namespace pe

@@ -112,7 +112,7 @@ def test_attention_needs_its_workspace(lib):
     assert lib.pe_paged_attn_fwd(ctypes.byref(a), None, size.value, None) == -3
     assert lib.pe_paged_attn_fwd(ctypes.byref(a), (1 << 20) + 4, size.value, None) == -3
     assert lib.pe_paged_workspace_size(ctypes.byref(a), None) == -1
-    short = _paged(max_seqlen_k=128)  # too few keys to spread
+    short = _paged(n_seq=1, total_tokens=1, max_seqlen_k=16)  # too few keys to spread
     assert lib.pe_paged_workspace_size(ctypes.byref(short), ctypes.byref(size)) == 0 and size.value == 0
 
 
