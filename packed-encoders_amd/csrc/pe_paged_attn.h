@@ -107,6 +107,14 @@ __device__ __forceinline__ bool reaches(const PagedParams &p, int pos, int key, 
     return key < khi && (p.wl < 0 || pos - key <= p.wl) && (p.wr < 0 || key - pos <= p.wr);
 }
 
+// `rows` rows from a page's `slot` on, of one head: a resource that ends with the last of them (rows <= 0: empty).
+// A page spans less than 2 GiB (the host checks), so that only its own place takes 64 bits.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const char *head, int page, uint64_t page_bytes, int slot,
+                                                            int row_bytes, int rows, int d) {
+    const char *first = head + (uint64_t)(uint32_t)page * page_bytes + (uint32_t)(slot * row_bytes);
+    return make_rsrc(first, rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)row_bytes + 2 * d : 0u);
+}
+
 // The 16 keys from `key` on (a multiple of 16) lie in a mapped page.
 __device__ __forceinline__ bool mapped16(const PagedParams &p, PageIds table, int key) {
     return (uint32_t)table[min(page_of(p, key), p.max_pages - 1)] < (uint32_t)p.n_pages;
@@ -204,7 +212,7 @@ __device__ __forceinline__ int64_t tile_slot(const PagedParams &p, int item, int
 // of 64 keys (32 at head_dim 256), filled by direct global-to-LDS loads of the next while the waves work on
 // one: 64 KB, two workgroups per CU (head_dim 64: three stages, 48 KB).
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedParams p) {
     constexpr int BM = kTileRows, BN = D == 256 ? 32 : 64, NS = D == 64 ? 3 : 2;
     constexpr int NB = BN / 32, DC = D / 16, DB = D / 32, CPR = D / 8;
     constexpr int TILE = BN * D, UPW = TILE / 8 / 64 / 4, LPS = 2 * UPW, KPW = BN / 4;
@@ -254,16 +262,16 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
         voff[j] = (key - wave * KPW) * v_row + ch * 16;
     }
     const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
+    const char *k_head = reinterpret_cast<const char *>(p.k + kvh * p.k_sh);
+    const char *v_head = reinterpret_cast<const char *>(p.v + kvh * p.v_sh);
+    const uint64_t k_page = 2 * p.k_sp, v_page = 2 * p.v_sp;
     auto page_id = [&](int step) { return table[min(page_of(p, klo + step * BN + wave * KPW), p.max_pages - 1)]; };
     auto issue = [&](int stage, int step, int id) {
         const int key0 = klo + step * BN + wave * KPW, slot = key0 - page_of(p, key0) * p.page;
         const bool mapped = (uint32_t)id < (uint32_t)p.n_pages;
         const int rows = mapped ? min(p.page - slot, t.lk - key0) : 0;
-        const int64_t page = mapped ? id : 0;
-        const __amdgpu_buffer_rsrc_t k_rs =
-            make_rsrc(p.k + page * p.k_sp + slot * p.k_st + kvh * p.k_sh, rows_bytes(rows, p.k_st, D));
-        const __amdgpu_buffer_rsrc_t v_rs =
-            make_rsrc(p.v + page * p.v_sp + slot * p.v_st + kvh * p.v_sh, rows_bytes(rows, p.v_st, D));
+        const __amdgpu_buffer_rsrc_t k_rs = page_rows(k_head, mapped ? id : 0, k_page, slot, k_row, rows, D);
+        const __amdgpu_buffer_rsrc_t v_rs = page_rows(v_head, mapped ? id : 0, v_page, slot, v_row, rows, D);
         const uint32_t kb = ring_base + stage * (4 * TILE) + wave * UPW * 1024, vb = kb + 2 * TILE;
         if constexpr (UPW == 2) {
             const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
@@ -300,6 +308,35 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
         for (int j = 0; j < 16; ++j) o[db][j] = 0.0f;
     float m = kNegInf, ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const float c2 = p.c;
+    auto values = [&](const __bf16 *keys, int db) {  // V^T of 16 keys, dims 32 db ..
+        const bf16x4 lo = tr16(keys + (vbase0 ^ (32 * db))), hi = tr16(keys + (vbase1 ^ (32 * db)));
+        return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto row_max = [](const auto &s) {
+        float mp[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+        for (const f32x16 &x : s)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mp[j & 3] = fmaxf(mp[j & 3], x[j]);
+        return fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3]));
+    };
+    // The maximum is raised only when a row exceeds it by 2^8: the exponentials stay in range and most steps
+    // skip the rescale. The two lanes of a row share m.
+    auto raise = [&](float mx) {
+        if (!wave_any(mx * c2 > m + 8.0f)) return;
+        const float mnew = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * c2);
+        const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m - mnew);
+        m = mnew;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ls[i] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[db][j] *= alpha;
+    };
+    // Steps of keys that all of the wave's rows reach and that lie in pages: [whole_from, whole_to).
+    const int whole_from = p.wl >= 0 ? p1 - 1 - p.wl : 0;
+    const int whole_to = any_hole ? 0 : p.wr < 0 || khi - 1 - p0 <= p.wr ? khi : p0 + 1 + p.wr;
 
     int next_id = 0;
     if (ntiles > 0) {
@@ -312,7 +349,7 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
     // loads ahead in every step.
 #pragma unroll
     for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[c]));
-    for (int step = 0; step < ntiles; ++step) {
+    auto arrive = [&](int step) {
         // The step's loads are complete once at most the later steps' are in flight.
         const int later = min(ntiles, step + NS - 1) - step - 1;
         if (NS >= 3 && later >= 1) wait_vmcnt<LPS>();
@@ -322,88 +359,90 @@ __global__ __launch_bounds__(256) void paged_tile_kernel(PagedParams p) {
             issue((step + NS - 1) % NS, step + NS - 1, next_id);
             next_id = page_id(step + NS);
         }
-        if (!wave_active) continue;
-        const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
-        const int kt0 = klo + step * BN;
-        f32x16 s[NB];
-        bool live[NB], whole[NB];
-        float mp[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+    };
+    auto scores = [&](const __bf16 *keys) {  // of 32 keys
+        f32x16 acc;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int kb0 = kt0 + 32 * b;
-            live[b] = block_live(kb0, khi, p0, p1, p.wl, p.wr);
-            whole[b] = true;
-            if (live[b]) {
-                f32x16 acc;
+        for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+        for (int c = 0; c < DC; ++c) acc = mfma32(ld_s16(keys + (kbase ^ (16 * c))), qf[c], acc);
+        return acc;
+    };
+    for (int step = 0; step < ntiles;) {
+        // A run of steps that need no mask: nothing but loads, products and the softmax.
+        const int first = klo + step * BN;
+        const int run_end = wave_active && first >= whole_from ? min(ntiles, step + max(0, whole_to - first) / BN) : step;
+        for (; step < run_end; ++step) {
+            arrive(step);
+            const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
+            f32x16 s[NB];
 #pragma unroll
-                for (int c = 0; c < DC; ++c) acc = mfma32(ld_s16(kt + 32 * b * D + (kbase ^ (16 * c))), qf[c], acc);
-                whole[b] = block_full(kb0, khi, p0, p1, p.wl, p.wr);
-                if (!whole[b] || any_hole) {
-                    uint32_t km = key_mask(kb0, kg, pos, khi, p.wl, p.wr);
-                    if (any_hole) {
-                        const uint32_t low = (1u << (16 - 4 * kg)) - 1u;  // bits of the block's first 16 keys
-                        km &= (mapped16(p, table, kb0) ? low : 0u) | (mapped16(p, table, kb0 + 16) ? ~low : 0u);
-                    }
+            for (int b = 0; b < NB; ++b) s[b] = scores(kt + 32 * b * D);
+            raise(row_max(s));
+            const float muse = m == kNegInf ? 0.0f : m;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[j] = mask_score(acc[j], km, acc_key(j, 0));
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[b][j] = exp2_fast(fmaf(s[b][j], c2, -muse));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 pb = to_bf16x8(s[b], 8 * h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ls[i] = sum2(pb, i, ls[i]);
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) o[db] = mfma32(values(vt + (32 * b + 16 * h) * D, db), pb, o[db]);
                 }
-                s[b] = acc;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mp[j & 3] = fmaxf(mp[j & 3], acc[j]);
             }
         }
-        // The maximum is raised only when a row exceeds it by 2^8: the exponentials stay in range and
-        // most tiles skip the rescale. The two lanes of a row share m.
-        const float mx = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3]));
-        if (wave_any(mx * c2 > m + 8.0f)) {
-            const float mnew = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * c2);
-            const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m - mnew);
-            m = mnew;
+        if (step >= ntiles) break;
+        arrive(step);
+        if (wave_active) {
+            const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
+            const int kt0 = klo + step * BN;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ls[i] *= alpha;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[db][j] *= alpha;
-        }
-        const float muse = m == kNegInf ? 0.0f : m;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (!live[b]) continue;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) s[b][j] = exp2_fast(fmaf(s[b][j], c2, -muse));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bf16x8 pb = to_bf16x8(s[b], 8 * h);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ls[i] = sum2(pb, i, ls[i]);
-                const __bf16 *vh = vt + (32 * b + 16 * h) * D;
-                auto values = [&](int db) {
-                    const bf16x4 lo = tr16(vh + (vbase0 ^ (32 * db))), hi = tr16(vh + (vbase1 ^ (32 * db)));
-                    return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                };
-                uint32_t bad = 0;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    bf16x8 va = values(db);
-                    if (!whole[b]) bad |= clean8(va);
-                    o[db] = mfma32(va, pb, o[db]);
+            for (int b = 0; b < NB; ++b) {
+                const int kb0 = kt0 + 32 * b;
+                if (!block_live(kb0, khi, p0, p1, p.wl, p.wr)) continue;
+                f32x16 s[1] = {scores(kt + 32 * b * D)};
+                uint32_t km = key_mask(kb0, kg, pos, khi, p.wl, p.wr);
+                if (any_hole) {
+                    const uint32_t low = (1u << (16 - 4 * kg)) - 1u;  // bits of the block's first 16 keys
+                    km &= (mapped16(p, table, kb0) ? low : 0u) | (mapped16(p, table, kb0 + 16) ? ~low : 0u);
                 }
-                if (!wave_any(bad != 0)) continue;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[0][j] = mask_score(s[0][j], km, acc_key(j, 0));
+                raise(row_max(s));
+                const float muse = m == kNegInf ? 0.0f : m;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[0][j] = exp2_fast(fmaf(s[0][j], c2, -muse));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 pb = to_bf16x8(s[0], 8 * h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ls[i] = sum2(pb, i, ls[i]);
+                    const __bf16 *vh = vt + (32 * b + 16 * h) * D;
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        bf16x8 va = values(vh, db);
+                        bad |= clean8(va);
+                        o[db] = mfma32(va, pb, o[db]);
+                    }
+                    if (!wave_any(bad != 0)) continue;
 #pragma unroll 1
-                for (int key = 0; key < 16; ++key) {
-                    const bool reach = reaches(p, pos, kt0 + 32 * b + 16 * h + key, khi);
+                    for (int key = 0; key < 16; ++key) {
+                        const bool reach = reaches(p, pos, kb0 + 16 * h + key, khi);
 #pragma unroll
-                    for (int q = 0; q < 4 * DB; ++q) {  // dims 8 q + 4 kg ..
-                        const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vh + key * D + (q ^ swz<CPR>(key)) * 8 + 4 * kg);
+                        for (int q = 0; q < 4 * DB; ++q) {  // dims 8 q + 4 kg ..
+                            const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vh + key * D + (q ^ swz<CPR>(key)) * 8 + 4 * kg);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[q >> 2][4 * (q & 3) + i] += reach ? only_nonfinite(v4[i]) : 0.0f;
+                            for (int i = 0; i < 4; ++i) o[q >> 2][4 * (q & 3) + i] += reach ? only_nonfinite(v4[i]) : 0.0f;
+                        }
                     }
                 }
             }
         }
+        ++step;
     }
     if (!wave_active) return;
     const float lsum = (ls[0] + ls[1]) + (ls[2] + ls[3]);
@@ -511,6 +550,9 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
     const int kbase = c16 * D + (g4 ^ swz<CPR>(c16)) * 8;
     const int vbase = vkey * D + ((vdim >> 3) ^ swz<CPR>(vkey)) * 8 + (vdim & 4);
     const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
+    const char *k_head = reinterpret_cast<const char *>(p.k + kvh * p.k_sh);
+    const char *v_head = reinterpret_cast<const char *>(p.v + kvh * p.v_sh);
+    const uint64_t k_page = 2 * p.k_sp, v_page = 2 * p.v_sp;
     const float c2 = p.c;
 
     int before = 0;  // steps of the sequences before seqs.base
@@ -545,12 +587,9 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
             for (int h = 0; h < 2; ++h) {
                 const int key0 = key_first + 32 * step + 16 * h, slot = key0 - page_of(p, key0) * p.page;
                 const int id = h ? ids.y : ids.x;
-                const int rows = mapped(id) ? max(0, min(p.page - slot, lk - key0)) : 0;
-                const int64_t page = mapped(id) ? id : 0;
-                const __amdgpu_buffer_rsrc_t k_rs =
-                    make_rsrc(p.k + page * p.k_sp + slot * p.k_st + kvh * p.k_sh, rows_bytes(rows, p.k_st, D));
-                const __amdgpu_buffer_rsrc_t v_rs =
-                    make_rsrc(p.v + page * p.v_sp + slot * p.v_st + kvh * p.v_sh, rows_bytes(rows, p.v_st, D));
+                const int rows = mapped(id) ? min(p.page - slot, lk - key0) : 0;
+                const __amdgpu_buffer_rsrc_t k_rs = page_rows(k_head, mapped(id) ? id : 0, k_page, slot, k_row, rows, D);
+                const __amdgpu_buffer_rsrc_t v_rs = page_rows(v_head, mapped(id) ? id : 0, v_page, slot, v_row, rows, D);
                 const uint32_t kb = base + h * LH * 1024, vb = kb + 2 * TILE;
                 if constexpr (LH == 2) {
                     const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
