@@ -82,7 +82,8 @@ struct PagedShape {
     int row_blocks;   // of 16 rows
     int32_t workers;  // waves per kv head
     int64_t tiles;    // items per kv head, at most
-    int32_t goal;     // workgroups its keys are split for, 0: not split
+    int32_t goal;     // whole chunks its keys are split into, 0: not split
+    int32_t chunk;    // steps of a chunk, 0: from goal
     int64_t run_slots, tile_slots;  // rows of parts, at most
 };
 
@@ -92,6 +93,31 @@ struct PagedShape {
 // 258 us (a fifth wave per CU waits for a second round), two of four 220 us; 64 users of 12 heads of 64: eight of
 // two stages 161 us, six of three 169 us, ten of two 182 us.
 int row_waves(int head_dim) { return head_dim == 64 ? 8 : head_dim == 128 ? 3 : 2; }
+
+// Steps of a chunk for a call of one sequence: its tiles, cut into c chunks each, run in rounds of `at_once`
+// workgroups (`most` items altogether), each as long as a chunk and what a workgroup costs beside (item, in steps of 64 keys), and the
+// parts are added (six steps' time per round). 512 new rows on 16,384 keys at 32:8 heads of 128, by rounds: 1
+// 154 us, 1.5 157, 2 163, 3 178; 700 rows 265, 208, 231, 222.
+int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t most) {
+    const int64_t item = a->head_dim == 64 ? 6 : a->head_dim == 128 ? 3 : 2;
+    const int wr = a->causal ? 0 : a->window_right;
+    int64_t reach = a->max_seqlen_k;
+    if (a->window_left >= 0 && wr >= 0) {
+        const int64_t band = (int64_t)a->window_left + wr + (pe::kTileRows - 1) / (a->n_heads_q / a->n_heads_kv) + 2 + 64;
+        if (band < reach) reach = band;
+    }
+    const int64_t steps = (reach + 63) / 64;
+    int64_t best = steps, least = (tiles + at_once - 1) / at_once * (steps + item);
+    for (int64_t c = 2; c * tiles <= most && c * pe::kChunkSteps <= steps; ++c) {
+        const int64_t chunk = (steps + c - 1) / c, items = c * tiles;
+        const int64_t cost = (items + at_once - 1) / at_once * (chunk + item) + 6 * items / at_once;
+        if (cost < least) {
+            least = cost;
+            best = chunk;
+        }
+    }
+    return (int32_t)best;
+}
 
 PagedShape paged_shape(const pe_paged_args *a) {
     PagedShape s;
@@ -117,16 +143,15 @@ PagedShape paged_shape(const pe_paged_args *a) {
     int64_t with = a->total_tokens * group / (s.few + 1);
     if (with > n) with = n;
     s.tiles = fill + with;
-    // Two workgroups per CU run at once (head_dim 256: one, for its registers). Calls of fewer tiles split
-    // their keys into about twice as many items.
-    const int64_t at_once = (a->head_dim == 256 ? 1 : 2) * kCUs;
+    // Two workgroups per CU run at once. Calls of fewer tiles split their keys.
+    const int64_t at_once = 2 * kCUs;
     if (fill * hkv < at_once && a->max_seqlen_k > 64 * pe::kChunkSteps) {
-        s.goal = (int32_t)(2 * at_once);
-        // Chunks hold at least 1 / goal of the work, so there are at most goal whole ones; a tile that is split
-        // has at most one that is not whole beside one that is.
+        s.goal = (int32_t)(a->head_dim == 256 ? 3 * at_once / 2 : 2 * at_once);  // (its parts are the largest)
+        // The even share makes at most goal whole chunks, and beside each at most one that is not.
         const int64_t longest = (a->max_seqlen_k + 64 * pe::kChunkSteps - 1) / (64 * pe::kChunkSteps) * s.tiles * hkv;
         s.tile_slots = (longest < 2 * s.goal ? longest : 2 * s.goal) * pe::kTileRows;
-        s.tiles += (s.goal + hkv - 1) / hkv;
+        if (n == 1) s.chunk = chunk_of(a, (rows + pe::kTileRows - 1) / pe::kTileRows * hkv, at_once, 2 * s.goal);
+        s.tiles += (2 * s.goal + hkv - 1) / hkv;
     }
     return s;
 }
@@ -169,6 +194,7 @@ pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *
     p.few = s.few;
     p.workers = s.workers;
     p.goal = s.goal;
+    p.chunk = s.chunk;
     p.tile_slots = s.run_slots;
     p.total_q = a->total_tokens;
     p.c = a->softmax_scale * pe::kLog2e;

@@ -28,7 +28,8 @@ struct PagedParams {
     int32_t max_seqlen, max_seqlen_k;
     int32_t few;                    // sequences of at most this many rows are paged_row_kernel's (0: none)
     int32_t workers;                // its waves per kv head
-    int32_t goal;                   // workgroups that paged_tile_kernel's items should come to, over the kv heads
+    int32_t goal;                   // whole chunks that paged_tile_kernel's keys should come to, over the kv heads
+    int32_t chunk;                  // steps of a chunk, 0: from goal
     int32_t total_q;
     float c;                        // softmax_scale * log2(e)
     int64_t tile_slots;             // first slot of paged_tile_kernel's parts
@@ -77,6 +78,14 @@ __device__ __forceinline__ void keys_of(const PagedParams &p, int off, int lk, i
     if (p.wr >= 0) khi = (int)max((int64_t)0, min((int64_t)lk, (int64_t)off + (row1 - 1) / p.group + 1 + p.wr));
 }
 
+// The 16-byte units of a row by key, as swz, but for rows of 512 bytes what it is for 256: the 32x32 operands'
+// transposing reads take 8 keys by 4 units, which key & 15 would lay on half of the banks (60 % of the
+// LDS cycles at head_dim 256 were conflicts). It depends on the key's low four bits alone.
+template <int CPR>
+__device__ __forceinline__ int unit_swz(int key) {
+    return swz<(CPR == 8 ? 8 : 16)>(key);
+}
+
 // A masked key may hold an infinity or NaN, whose product with a zero probability is NaN. In blocks that
 // not every row reaches whole, the products therefore run on values cleaned of them (clean8, which tells
 // whether there was one), and where one was found each row that reaches it takes it by itself: a
@@ -122,9 +131,8 @@ __device__ __forceinline__ bool mapped16(const PagedParams &p, PageIds table, in
 
 // ----------------------------------------------------------------------------- many rows
 
-// Items of paged_tile_kernel: a query tile of 128 rows over a chunk of its keys. The chunk is as long as brings
-// the call to about `goal` workgroups: few tiles are split until they fill the chip, many stay whole, and
-// sequences of any lengths are cut alike. Every wave works this out from the bounds, 64 sequences at a time.
+// Items of paged_tile_kernel: a query tile of 128 rows over a chunk of its keys. Calls of few tiles split their
+// keys until they fill the chip, many tiles stay whole; sequences of any lengths are cut alike.
 constexpr int kTileRows = 128;
 constexpr int kChunkSteps = 4;  // of 64 keys, at least
 
@@ -143,8 +151,17 @@ __device__ __forceinline__ TileLanes tile_lanes(const PagedParams &p, int base) 
     return t;
 }
 
-// Steps of a chunk (SPLIT calls).
+// The chunks of a sequence's tiles, at most; and its items that leave parts, one for each chunk of a tile.
+__device__ __forceinline__ int chunks_of(const TileLanes &t, int steps) { return max(1, (t.reach + steps - 1) / steps); }
+__device__ __forceinline__ int split_items(const TileLanes &t, int steps) {
+    const int n = chunks_of(t, steps);
+    return n > 1 ? t.tiles * n : 0;
+}
+
+// Steps of a chunk (SPLIT calls): the host's choice for a call of one sequence, whose work it knows, else the
+// even share of all the call's work. Every wave works it out alike, from the bounds alone.
 __device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes &first) {
+    if (p.chunk > 0) return p.chunk;
     uint64_t sum = (uint64_t)first.tiles * first.reach;
     for (int base = 64; base < p.n_seq; base += 64) {
         const TileLanes t = tile_lanes(p, base);
@@ -154,13 +171,6 @@ __device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((unsigned long long)sum, d);
     const uint64_t steps = (sum * p.hkv + p.goal - 1) / p.goal;
     return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 25)));
-}
-
-// The chunks of a sequence's tiles, at most; and its items that leave parts, one for each chunk of a tile.
-__device__ __forceinline__ int chunks_of(const TileLanes &t, int steps) { return max(1, (t.reach + steps - 1) / steps); }
-__device__ __forceinline__ int split_items(const TileLanes &t, int steps) {
-    const int n = chunks_of(t, steps);
-    return n > 1 ? t.tiles * n : 0;
 }
 
 struct TileItem {
@@ -212,7 +222,7 @@ __device__ __forceinline__ int64_t tile_slot(const PagedParams &p, int item, int
 // of 64 keys (32 at head_dim 256), filled by direct global-to-LDS loads of the next while the waves work on
 // one: 64 KB, two workgroups per CU (head_dim 64: three stages, 48 KB).
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
     constexpr int BM = kTileRows, BN = D == 256 ? 32 : 64, NS = D == 64 ? 3 : 2;
     constexpr int NB = BN / 32, DC = D / 16, DB = D / 32, CPR = D / 8;
     constexpr int TILE = BN * D, UPW = TILE / 8 / 64 / 4, LPS = 2 * UPW, KPW = BN / 4;
@@ -257,7 +267,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(Paged
 #pragma unroll
     for (int j = 0; j < UPW; ++j) {
         const int u = (wave * UPW + j) * 64 + lane;
-        const int key = u / CPR, ch = (u % CPR) ^ swz<CPR>(key);
+        const int key = u / CPR, ch = (u % CPR) ^ unit_swz<CPR>(key);
         koff[j] = (key - wave * KPW) * k_row + ch * 16;
         voff[j] = (key - wave * KPW) * v_row + ch * 16;
     }
@@ -297,9 +307,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(Paged
     // Place of the operands' first chunk in a stage: chunk c of K is 16 c elements on, block db of V^T 32 db,
     // by exclusive or (the swizzle exchanges whole units of a row).
     const int vkey = 4 * kg + ((lane & 15) >> 2), vdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const int kbase = col * D + (kg ^ swz<CPR>(col)) * 8;
-    const int vbase0 = vkey * D + ((vdim >> 3) ^ swz<CPR>(vkey)) * 8 + (vdim & 4);
-    const int vbase1 = (vkey + 8) * D + ((vdim >> 3) ^ swz<CPR>(vkey + 8)) * 8 + (vdim & 4);
+    int kbase = col * D + (kg ^ unit_swz<CPR>(col)) * 8;
+    int vbase0 = vkey * D + ((vdim >> 3) ^ unit_swz<CPR>(vkey)) * 8 + (vdim & 4);
+    int vbase1 = (vkey + 8) * D + ((vdim >> 3) ^ unit_swz<CPR>(vkey + 8)) * 8 + (vdim & 4);
 
     f32x16 o[DB];
 #pragma unroll
@@ -374,6 +384,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(Paged
         const int run_end = wave_active && first >= whole_from ? min(ntiles, step + max(0, whole_to - first) / BN) : step;
         for (; step < run_end; ++step) {
             arrive(step);
+            if constexpr (D == 256) asm volatile("" : "+v"(kbase), "+v"(vbase0), "+v"(vbase1));
             const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
             f32x16 s[NB];
 #pragma unroll
@@ -434,7 +445,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(Paged
                         const bool reach = reaches(p, pos, kb0 + 16 * h + key, khi);
 #pragma unroll
                         for (int q = 0; q < 4 * DB; ++q) {  // dims 8 q + 4 kg ..
-                            const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vh + key * D + (q ^ swz<CPR>(key)) * 8 + 4 * kg);
+                            const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vh + key * D + (q ^ unit_swz<CPR>(key)) * 8 + 4 * kg);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[q >> 2][4 * (q & 3) + i] += reach ? only_nonfinite(v4[i]) : 0.0f;
                         }
@@ -540,15 +551,15 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
     int koff[LH], voff[LH];
 #pragma unroll
     for (int j = 0; j < LH; ++j) {
-        const int u = j * 64 + lane, key = u / CPR, ch = (u % CPR) ^ swz<CPR>(key);
+        const int u = j * 64 + lane, key = u / CPR, ch = (u % CPR) ^ unit_swz<CPR>(key);
         koff[j] = key * k_row + ch * 16;
         voff[j] = key * v_row + ch * 16;
     }
     // Place of the operands' first chunk in a stage; the swizzle exchanges whole units and depends on the
     // key's low four bits alone, so chunk c is 32 c elements on by exclusive or, and 16 keys on by sum.
     const int vkey = 4 * g4 + (c16 >> 2), vdim = 4 * (c16 & 3);
-    const int kbase = c16 * D + (g4 ^ swz<CPR>(c16)) * 8;
-    const int vbase = vkey * D + ((vdim >> 3) ^ swz<CPR>(vkey)) * 8 + (vdim & 4);
+    const int kbase = c16 * D + (g4 ^ unit_swz<CPR>(c16)) * 8;
+    const int vbase = vkey * D + ((vdim >> 3) ^ unit_swz<CPR>(vkey)) * 8 + (vdim & 4);
     const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
     const char *k_head = reinterpret_cast<const char *>(p.k + kvh * p.k_sh);
     const char *v_head = reinterpret_cast<const char *>(p.v + kvh * p.v_sh);
@@ -728,7 +739,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
                 for (int key = 0; key < BN; ++key) {
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {  // dims 16 db + 4 g4 ..
-                        const int unit = (2 * db + (g4 >> 1)) ^ swz<CPR>(key);
+                        const int unit = (2 * db + (g4 >> 1)) ^ unit_swz<CPR>(key);
                         const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vt + key * D + unit * 8 + 4 * (g4 & 1));
 #pragma unroll
                         for (int r = 0; r < NR; ++r) {

@@ -118,10 +118,13 @@ def test_attention_needs_its_workspace(lib):
 
 def test_workspace_stays_bounded(lib):
     size = ctypes.c_size_t(0)
-    for n, tokens, longest, keys in [(1, 1, 1, 1 << 30), (1, 4096, 4096, 1 << 20), (300, 300, 1, 1 << 17), (8, 60000, 9000, 9000)]:
-        a = _paged(n_seq=n, total_tokens=tokens, max_seqlen=longest, max_seqlen_k=keys)
-        assert lib.pe_paged_workspace_size(ctypes.byref(a), ctypes.byref(size)) == 0
-        assert size.value <= 256 << 20
+    for n, tokens, longest, keys in [(1, 1, 1, 1 << 30), (1, 4096, 4096, 1 << 20), (300, 300, 1, 1 << 17), (8, 60000, 9000, 9000),
+                                    (40, 700, 300, 30000), (2, 33, 32, 1 << 20)]:
+        for hq, hkv, d in [(32, 8, 128), (8, 2, 256), (64, 64, 256), (12, 12, 64), (48, 1, 256), (640, 640, 256), (9000, 9000, 64)]:
+            a = _paged(n_seq=n, total_tokens=tokens, max_seqlen=longest, max_seqlen_k=keys, n_heads_q=hq, n_heads_kv=hkv,
+                       head_dim=d)
+            assert lib.pe_paged_workspace_size(ctypes.byref(a), ctypes.byref(size)) == 0
+            assert size.value <= 256 << 20, (n, tokens, longest, keys, hq, hkv, d)
 
 
 def test_empty_calls_launch_nothing(lib):
