@@ -147,11 +147,17 @@ PagedShape paged_shape(const pe_paged_args *a) {
     const int64_t at_once = 2 * kCUs;
     if (fill * hkv < at_once && a->max_seqlen_k > 64 * pe::kChunkSteps) {
         s.goal = (int32_t)(a->head_dim == 256 ? 3 * at_once / 2 : 2 * at_once);  // (its parts are the largest)
-        // The even share makes at most goal whole chunks, and beside each at most one that is not.
-        const int64_t longest = (a->max_seqlen_k + 64 * pe::kChunkSteps - 1) / (64 * pe::kChunkSteps) * s.tiles * hkv;
-        s.tile_slots = (longest < 2 * s.goal ? longest : 2 * s.goal) * pe::kTileRows;
-        if (n == 1) s.chunk = chunk_of(a, (rows + pe::kTileRows - 1) / pe::kTileRows * hkv, at_once, 2 * s.goal);
-        s.tiles += (2 * s.goal + hkv - 1) / hkv;
+        // The even share makes at most goal whole chunks, and one that is not of every tile; parts are left by
+        // tiles of two chunks and more, so by at most 2 * goal.
+        int64_t items = s.tiles + (s.goal + hkv - 1) / hkv;
+        int64_t longest = s.tiles * ((a->max_seqlen_k + 64 * pe::kChunkSteps - 1) / (64 * pe::kChunkSteps));
+        if (n == 1) {
+            const int64_t tiles = (rows + pe::kTileRows - 1) / pe::kTileRows;
+            s.chunk = chunk_of(a, tiles * hkv, at_once, 2 * s.goal);
+            items = longest = tiles * ((a->max_seqlen_k + 64 * s.chunk - 1) / (64 * (int64_t)s.chunk));
+        }
+        s.tiles = items < longest ? items : longest;
+        s.tile_slots = (longest * hkv < 2 * s.goal ? longest * hkv : 2 * s.goal) * pe::kTileRows;
     }
     return s;
 }
@@ -187,6 +193,8 @@ pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *
     p.page = a->page_size;
     p.max_pages = a->max_pages;
     divider((uint32_t)a->page_size, &p.page_mul, &p.page_shift);
+    if (p.group > 1) divider((uint32_t)p.group, &p.group_mul, &p.group_shift);
+    if (p.hkv > 1) divider((uint32_t)p.hkv, &p.hkv_mul, &p.hkv_shift);
     p.wl = a->window_left;
     p.wr = a->causal ? 0 : a->window_right;
     p.max_seqlen = a->max_seqlen;

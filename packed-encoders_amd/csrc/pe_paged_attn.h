@@ -23,7 +23,8 @@ struct PagedParams {
     int64_t q_st, q_sh, k_sp, k_st, k_sh, v_sp, v_st, v_sh, o_st, o_sh, table_st;
     int32_t n_seq, hq, hkv, group;
     int32_t n_pages, page, max_pages;
-    uint32_t page_mul, page_shift;  // n / page = (n * page_mul >> 32) >> page_shift for 0 <= n < 2^31
+    // n / d = (n * mul >> 32) >> shift for 0 <= n < 2^31 (d > 1; group_mul 0: a group of one)
+    uint32_t page_mul, page_shift, group_mul, group_shift, hkv_mul, hkv_shift;
     int32_t wl, wr;                 // window (-1: unbounded); causal folded into wr = 0
     int32_t max_seqlen, max_seqlen_k;
     int32_t few;                    // sequences of at most this many rows are paged_row_kernel's (0: none)
@@ -38,6 +39,15 @@ struct PagedParams {
 
 __device__ __forceinline__ int page_of(const PagedParams &p, int key) {
     return (int)(__umulhi((uint32_t)key, p.page_mul) >> p.page_shift);
+}
+
+// Token of a sequence's row (token * group + head of the kv head).
+__device__ __forceinline__ int token_of(const PagedParams &p, int row) {
+    return p.group_mul ? (int)(__umulhi((uint32_t)row, p.group_mul) >> p.group_shift) : row;
+}
+
+__device__ __forceinline__ int over_kv_heads(const PagedParams &p, int n) {
+    return p.hkv_mul ? (int)(__umulhi((uint32_t)n, p.hkv_mul) >> p.hkv_shift) : n;
 }
 
 // The page table as constant memory: a wave's uniform entry is then a scalar load, which the waits for its
@@ -73,9 +83,9 @@ __device__ __forceinline__ Lanes lanes_from(const PagedParams &p, int base) {
 // Keys [klo, khi) that some of the rows [row0, row1) of a sequence reach by position, klo on a multiple of 64.
 // `off` is the key position of its first new token.
 __device__ __forceinline__ void keys_of(const PagedParams &p, int off, int lk, int row0, int row1, int &klo, int &khi) {
-    klo = p.wl >= 0 ? max(0, off + row0 / p.group - p.wl) & ~63 : 0;
+    klo = p.wl >= 0 ? max(0, off + token_of(p, row0) - p.wl) & ~63 : 0;
     khi = lk;
-    if (p.wr >= 0) khi = (int)max((int64_t)0, min((int64_t)lk, (int64_t)off + (row1 - 1) / p.group + 1 + p.wr));
+    if (p.wr >= 0) khi = (int)max((int64_t)0, min((int64_t)lk, (int64_t)off + token_of(p, row1 - 1) + 1 + p.wr));
 }
 
 // The 16-byte units of a row by key, as swz, but for rows of 512 bytes what it is for 256: the 32x32 operands'
@@ -146,7 +156,7 @@ __device__ __forceinline__ TileLanes tile_lanes(const PagedParams &p, int base) 
     t.seq = lanes_from(p, base);
     t.tiles = t.seq.rows > p.few ? (t.seq.rows + kTileRows - 1) / kTileRows : 0;
     int64_t keys = t.seq.lk;
-    if (p.wl >= 0 && p.wr >= 0) keys = min(keys, (int64_t)p.wl + p.wr + (kTileRows - 1) / p.group + 2 + 64);
+    if (p.wl >= 0 && p.wr >= 0) keys = min(keys, (int64_t)p.wl + p.wr + token_of(p, kTileRows - 1) + 2 + 64);
     t.reach = (int)((keys + 63) >> 6);
     return t;
 }
@@ -162,14 +172,17 @@ __device__ __forceinline__ int split_items(const TileLanes &t, int steps) {
 // even share of all the call's work. Every wave works it out alike, from the bounds alone.
 __device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes &first) {
     if (p.chunk > 0) return p.chunk;
-    uint64_t sum = (uint64_t)first.tiles * first.reach;
-    for (int base = 64; base < p.n_seq; base += 64) {
-        const TileLanes t = tile_lanes(p, base);
-        sum += (uint64_t)t.tiles * t.reach;
+    // The lanes' products, below 2^47 each, summed in two parts of 32 bits.
+    uint64_t sum = 0;
+    for (int base = 0; base < p.n_seq; base += 64) {
+        const TileLanes t = base ? tile_lanes(p, base) : first;
+        const uint64_t work = (uint64_t)(uint32_t)t.tiles * (uint32_t)t.reach;
+        const uint32_t low = __builtin_amdgcn_readlane(wave_scan((int)(work & 0xffffff)), 63);
+        const uint32_t high = __builtin_amdgcn_readlane(wave_scan((int)(work >> 24)), 63);
+        sum += ((uint64_t)high << 24) + low;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((unsigned long long)sum, d);
-    const uint64_t steps = (sum * p.hkv + p.goal - 1) / p.goal;
+    sum = sum * p.hkv + p.goal - 1;
+    const uint64_t steps = sum >> 32 ? sum / p.goal : (uint64_t)((uint32_t)sum / (uint32_t)p.goal);
     return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 25)));
 }
 
@@ -197,7 +210,7 @@ __device__ __forceinline__ TileItem find_item(const PagedParams &p, int entry, i
             it.start = __builtin_amdgcn_readlane(t.seq.start, who);
             it.rows = __builtin_amdgcn_readlane(t.seq.rows, who);
             it.lk = __builtin_amdgcn_readlane(t.seq.lk, who);
-            it.off = it.lk - it.rows / p.group;
+            it.off = it.lk - token_of(p, it.rows);
             it.chunk = SPLIT ? at / tiles : 0;  // a chunk's tiles side by side: they read the same keys
             it.row0 = (at - it.chunk * tiles) * kTileRows;
             if constexpr (SPLIT)
@@ -229,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
     static_assert(UPW == 2 || UPW == 4, "loads go out four at a time");
     __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
 
-    const int entry = blockIdx.x / p.hkv, kvh = blockIdx.x - entry * p.hkv;
+    const int entry = over_kv_heads(p, blockIdx.x), kvh = blockIdx.x - entry * p.hkv;
     int steps = 0;
     const TileItem t = find_item<SPLIT>(p, entry, steps);
     if (!t.valid) return;
@@ -247,10 +260,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
     const int col = lane & 31, kg = lane >> 5;
     const int r0 = t.row0 + 32 * wave, row = r0 + col;
     const bool wave_active = r0 < t.rows;
-    const int token = row / p.group, head = kvh * p.group + row - token * p.group;
+    const int token = token_of(p, row), head = kvh * p.group + row - token * p.group;
     const int pos = t.off + token;  // the row's key position
     // Key positions of the wave's first row and past its last.
-    const int p0 = t.off + r0 / p.group, p1 = t.off + (min(t.rows, r0 + 32) - 1) / p.group + 1;
+    const int p0 = t.off + token_of(p, r0), p1 = t.off + token_of(p, min(t.rows, r0 + 32) - 1) + 1;
 
     const PageIds table = page_ids_of(p, t.seq);
     // Whether some page of the workgroup's keys is unmapped (its blocks then look again).
@@ -477,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     const __amdgpu_buffer_rsrc_t o_rs =
         make_rsrc(p.o + (int64_t)t.start * p.o_st,
-                  (uint32_t)(((int64_t)(t.rows / p.group - 1) * p.o_st + (p.hq - 1) * p.o_sh + D) * 2));
+                  (uint32_t)(((int64_t)(token_of(p, t.rows) - 1) * p.o_st + (p.hq - 1) * p.o_sh + D) * 2));
     const int ooff = row < t.rows ? (int)((token * p.o_st + head * p.o_sh) * 2) : kVoidOffset;
     store_block<DB, false>(o, inv, kg, o_rs, ooff, o_rs, 0);
 }
@@ -503,7 +516,7 @@ __device__ __forceinline__ RowLanes row_lanes(const PagedParams &p, int base) {
     r.n = 0;
     if (r.seq.rows > 0 && r.seq.rows <= p.few) {
         int klo, khi;
-        keys_of(p, r.seq.lk - r.seq.rows / p.group, r.seq.lk, 0, r.seq.rows, klo, khi);
+        keys_of(p, r.seq.lk - token_of(p, r.seq.rows), r.seq.lk, 0, r.seq.rows, klo, khi);
         r.n = max(1, (khi - klo + 31) >> 5);  // a sequence without a key in reach still has rows to write
     }
     r.upto = wave_scan(r.n);
@@ -538,7 +551,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
     static_assert(LH == 2 || LH % 4 == 0, "loads go out four at a time");
     __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
 
-    const int kvh = blockIdx.x % p.hkv, worker = blockIdx.x / p.hkv;
+    const int worker = over_kv_heads(p, blockIdx.x), kvh = blockIdx.x - worker * p.hkv;
     const int lane = threadIdx.x, c16 = lane & 15, g4 = lane >> 4;
     RowLanes seqs = row_lanes(p, 0);
     int total = seqs.all;
@@ -576,7 +589,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
         const int begin = before + __builtin_amdgcn_readlane(seqs.upto - seqs.n, who);
         const int end = before + __builtin_amdgcn_readlane(seqs.upto, who);
         const int start = __builtin_amdgcn_readlane(seqs.seq.start, who), nrows = __builtin_amdgcn_readlane(seqs.seq.rows, who);
-        const int lk = __builtin_amdgcn_readlane(seqs.seq.lk, who), off = lk - nrows / p.group;
+        const int lk = __builtin_amdgcn_readlane(seqs.seq.lk, who), off = lk - token_of(p, nrows);
         int klo, khi;
         keys_of(p, off, lk, 0, nrows, klo, khi);
         const int key_first = klo + 32 * (x - begin), steps = min(last, end) - x;
@@ -628,13 +641,13 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
         bf16x8 qf[NR][DC];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int row = 16 * r + c16, token = row / p.group, head = kvh * p.group + row - token * p.group;
+            const int row = 16 * r + c16, token = token_of(p, row), head = kvh * p.group + row - token * p.group;
             pos[r] = off + token;
             const __bf16 *src = p.q + (int64_t)(start + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g4;
 #pragma unroll
             for (int c = 0; c < DC; ++c) qf[r][c] = row < nrows ? ld_g16(src + 32 * c) : bf16x8{};
         }
-        const int p0 = off, p1 = off + (nrows - 1) / p.group + 1;  // key positions of the first row, past the last
+        const int p0 = off, p1 = off + token_of(p, nrows - 1) + 1;  // key positions of the first row, past the last
 
         f32x4 o[NR][DB];
         float m[NR], ls[NR];
@@ -758,7 +771,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
             const int row = 16 * r + c16;
             if (row >= nrows) continue;
             if (whole_row) {
-                const int token = row / p.group, head = kvh * p.group + row - token * p.group;
+                const int token = token_of(p, row), head = kvh * p.group + row - token * p.group;
                 const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
                 __bf16 *dst = p.o + (int64_t)(start + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g4;
 #pragma unroll
@@ -809,7 +822,7 @@ __device__ __forceinline__ RowPlace row_place(const PagedParams &p, int row) {
     for (int base = 0; base < p.n_seq; base += 64) {
         const TileLanes t = tile_lanes(p, base);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(t.seq.rows > 0 && t.seq.start <= row &&
-                                                         row < t.seq.start + t.seq.rows / p.group);
+                                                         row < t.seq.start + token_of(p, t.seq.rows));
         const bool here = hit && r.token < 0;
         const int who = here ? __builtin_ctzll(hit) : 0;
         if (here) {
@@ -845,7 +858,7 @@ __device__ __forceinline__ RowParts parts_of(const PagedParams &p, const RowPlac
     RowParts s;
     s.count = 0;
     s.first = s.rest = s.step = 0;
-    const int kvh = qh / p.group, at = r.token * p.group + qh - kvh * p.group;  // row of the sequence
+    const int kvh = token_of(p, qh), at = r.token * p.group + qh - kvh * p.group;  // row of the sequence
     if (r.token < 0) return s;
     if (RUNS && r.rows <= p.few) {
         const int w0 = r.begin / r.run;
@@ -856,7 +869,7 @@ __device__ __forceinline__ RowParts parts_of(const PagedParams &p, const RowPlac
     } else if (TILES && r.rows > p.few) {
         const int tile = at / kTileRows;
         int klo, khi;
-        keys_of(p, r.lk - r.rows / p.group, r.lk, tile * kTileRows, min(r.rows, (tile + 1) * kTileRows), klo, khi);
+        keys_of(p, r.lk - token_of(p, r.rows), r.lk, tile * kTileRows, min(r.rows, (tile + 1) * kTileRows), klo, khi);
         s.count = max(0, khi - klo + 64 * r.steps - 1) / (64 * r.steps);
         s.first = s.rest = tile_slot(p, r.item0 + tile, kvh) + at - tile * kTileRows;
         s.step = (int64_t)r.tiles * p.hkv * kTileRows;

@@ -131,6 +131,17 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     or beyond ``cu_seqlens[-1]``, and those of a sequence past its bounds or its table, are not written.
     Forward only. Calls of few query rows spread long key ranges over the chip and add the parts in a fixed
     order: results do not change from run to run, but their rounding may with the batch."""
+    native = native_for(q)  # first: it serves nothing that the checks below would refuse
+    if native is not None and isinstance(k_pages, Tensor) and isinstance(page_table, Tensor):
+        held = max_seqlen_k
+        if held is None and k_pages.ndim == 4 and page_table.ndim == 2:
+            held = min(page_table.shape[1] * k_pages.shape[1], 1 << 30)
+        scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+        out = None if held is None else native.paged_attention(
+            q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, max_seqlen, held, scale, window[0], window[1],
+            bool(causal))
+        if out is not None:
+            return out
     _no_grad("paged attention", q, k_pages, v_pages)
     _on_device("paged attention", q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k)
     if page_table.ndim != 2 or k_pages.ndim != 4:
@@ -139,11 +150,6 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
         max_seqlen_k = min(page_table.shape[1] * k_pages.shape[1], 1 << 30)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     options = (int(max_seqlen), int(max_seqlen_k), scale, int(window[0]), int(window[1]), bool(causal))
-    native = native_for(q)
-    if native is not None:
-        out = native.paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, *options)
-        if out is not None:
-            return out
     return torch.ops.pe_hip.paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, *options)
 
 
@@ -209,14 +215,15 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
     Rows whose position is negative or lies in no mapped page are dropped; rows at or beyond
     ``cu_seqlens[-1]`` are left alone (q's too). Sequences that append in one call need last pages of their
     own (``PagedCache`` sees to it). Forward only."""
+    native = native_for(k)  # first: it serves nothing that the checks below would refuse
+    if native is not None:
+        done = native.paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, inv_freq,
+                                   bool(interleaved), rope_scale)
+        if done is not None:
+            return done if q is not None else None
     _no_grad("paged_append", q, k, v, k_pages, v_pages, inv_freq)
     _on_device("paged_append", q, k, v, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, inv_freq)
     options = (inv_freq, bool(interleaved), float(rope_scale))
-    native = native_for(k)
-    if native is not None:
-        done = native.paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, *options)
-        if done is not None:
-            return done if q is not None else None
     out = torch.ops.pe_hip.paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, *options)
     return out[0] if q is not None else None
 
@@ -281,14 +288,14 @@ def copy_pages(pages: Tensor | Sequence[Tensor], src: Sequence[int], dst: Sequen
     target of one pair at most and then no source. ``ValueError`` otherwise, with nothing copied. Every
     page is one dense piece of memory, in 16-byte steps."""
     tensors = [pages] if isinstance(pages, Tensor) else list(pages)
-    src, dst = [int(x) for x in src], [int(x) for x in dst]
     if not tensors:
         raise ValueError("copy_pages needs a cache")
-    _no_grad("copy_pages", *tensors)
-    _on_device("copy_pages", *tensors)
-    native = native_for(tensors[0])
+    native = native_for(tensors[0])  # first: it serves nothing that the checks below would refuse
     if native is not None and native.copy_pages(tensors, src, dst):
         return
+    src, dst = [int(x) for x in src], [int(x) for x in dst]
+    _no_grad("copy_pages", *tensors)
+    _on_device("copy_pages", *tensors)
     torch.ops.pe_hip.copy_pages(tensors, src, dst)
 
 
