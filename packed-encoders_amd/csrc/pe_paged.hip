@@ -130,7 +130,8 @@ PagedShape paged_shape(const pe_paged_args *a) {
     if ((rows <= 32 || (uneven && group <= 16)) && steps < (int64_t)1 << 30) {
         s.few = rows > 16 && rows <= 32 ? 32 : 16;
         s.row_blocks = s.few / 16;
-        int64_t workers = row_waves(a->head_dim) * kCUs / hkv;
+        const int waves = rows <= 32 ? row_waves(a->head_dim) : a->head_dim == 64 ? 4 : a->head_dim == 128 ? 2 : 1;
+        int64_t workers = waves * kCUs / hkv;
         const int64_t most = (steps + pe::kRunSteps - 1) / pe::kRunSteps;
         if (workers > most) workers = most;
         if (workers > pe::kMaxParts) workers = pe::kMaxParts;
@@ -229,23 +230,27 @@ int launch_merge(const pe_paged_args *a, const pe::PagedParams &p, hipStream_t s
 template <int D>
 int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedParams &p, hipStream_t stream) {
     const int64_t blocks = s.tiles * a->n_heads_kv;
-    if (blocks > 0x7fffffffLL || (int64_t)a->total_tokens * a->n_heads_q > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
-    if (s.row_blocks) {
+    if (blocks > 0x7fffff00LL - 8 * kCUs || (int64_t)a->total_tokens * a->n_heads_q > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    if (s.row_blocks && s.tiles) {
+        const int groups = (int)((s.workers * a->n_heads_kv + pe::kRowWaves<D> - 1) / pe::kRowWaves<D>);
+        const dim3 grid((unsigned)(blocks + groups));
+        if (s.goal)
+            hipLaunchKernelGGL((pe::paged_both_kernel<D, true>), grid, dim3(256), 0, stream, p, groups);
+        else
+            hipLaunchKernelGGL((pe::paged_both_kernel<D, false>), grid, dim3(256), 0, stream, p, groups);
+    } else if (s.row_blocks) {
         constexpr int NS = D == 128 ? 3 : 2;
         const dim3 grid((unsigned)(s.workers * a->n_heads_kv));
         if (s.row_blocks == 1)
             hipLaunchKernelGGL((pe::paged_row_kernel<D, 1, NS>), grid, dim3(64), 0, stream, p);
         else
             hipLaunchKernelGGL((pe::paged_row_kernel<D, 2, NS>), grid, dim3(64), 0, stream, p);
-        if (const int status = launched()) return status;
+    } else if (s.goal) {
+        hipLaunchKernelGGL((pe::paged_tile_kernel<D, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    } else {
+        hipLaunchKernelGGL((pe::paged_tile_kernel<D, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     }
-    if (s.tiles) {
-        if (s.goal)
-            hipLaunchKernelGGL((pe::paged_tile_kernel<D, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-        else
-            hipLaunchKernelGGL((pe::paged_tile_kernel<D, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-        if (const int status = launched()) return status;
-    }
+    if (const int status = launched()) return status;
     if (s.run_slots && s.tile_slots) return launch_merge<D, true, true>(a, p, stream);
     if (s.run_slots) return launch_merge<D, true, false>(a, p, stream);
     if (s.tile_slots) return launch_merge<D, false, true>(a, p, stream);

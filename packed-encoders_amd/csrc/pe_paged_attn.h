@@ -234,15 +234,18 @@ __device__ __forceinline__ int64_t tile_slot(const PagedParams &p, int item, int
 // Four waves of 32 rows over keys that all of them read from LDS: chunks of prompts, and any call. Two stages
 // of 64 keys (32 at head_dim 256), filled by direct global-to-LDS loads of the next while the waves work on
 // one: 64 KB, two workgroups per CU (head_dim 64: three stages, 48 KB).
+template <int D>
+constexpr int kTileStages = D == 64 ? 3 : 2;
+template <int D>
+constexpr int kTileLds = kTileStages<D> * 2 * (D == 256 ? 32 : 64) * D;  // elements
+
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
-    constexpr int BM = kTileRows, BN = D == 256 ? 32 : 64, NS = D == 64 ? 3 : 2;
+__device__ __forceinline__ void tile_item(const PagedParams &p, int block, __bf16 *ring) {
+    constexpr int BM = kTileRows, BN = D == 256 ? 32 : 64, NS = kTileStages<D>;
     constexpr int NB = BN / 32, DC = D / 16, DB = D / 32, CPR = D / 8;
     constexpr int TILE = BN * D, UPW = TILE / 8 / 64 / 4, LPS = 2 * UPW, KPW = BN / 4;
     static_assert(UPW == 2 || UPW == 4, "loads go out four at a time");
-    __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
-
-    const int entry = over_kv_heads(p, blockIdx.x), kvh = blockIdx.x - entry * p.hkv;
+    const int entry = over_kv_heads(p, block), kvh = block - entry * p.hkv;
     int steps = 0;
     const TileItem t = find_item<SPLIT>(p, entry, steps);
     if (!t.valid) return;
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
         koff[j] = (key - wave * KPW) * k_row + ch * 16;
         voff[j] = (key - wave * KPW) * v_row + ch * 16;
     }
-    const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
+    const uint32_t ring_base = uniform((int)lds_addr(ring));
     const char *k_head = reinterpret_cast<const char *>(p.k + kvh * p.k_sh);
     const char *v_head = reinterpret_cast<const char *>(p.v + kvh * p.v_sh);
     const uint64_t k_page = 2 * p.k_sp, v_page = 2 * p.v_sp;
@@ -398,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
         for (; step < run_end; ++step) {
             arrive(step);
             if constexpr (D == 256) asm volatile("" : "+v"(kbase), "+v"(vbase0), "+v"(vbase1));
-            const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
+            const __bf16 *kt = ring + step % NS * (2 * TILE), *vt = kt + TILE;
             f32x16 s[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) s[b] = scores(kt + 32 * b * D);
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
         if (step >= ntiles) break;
         arrive(step);
         if (wave_active) {
-            const __bf16 *kt = &ring[step % NS][0][0], *vt = &ring[step % NS][1][0];
+            const __bf16 *kt = ring + step % NS * (2 * TILE), *vt = kt + TILE;
             const int kt0 = klo + step * BN;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -495,6 +498,12 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
     store_block<DB, false>(o, inv, kg, o_rs, ooff, o_rs, 0);
 }
 
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedParams p) {
+    __shared__ __attribute__((aligned(16))) __bf16 ring[kTileLds<D>];
+    tile_item<D, SPLIT>(p, blockIdx.x, ring);
+}
+
 // ----------------------------------------------------------------------------- few rows
 
 // Calls of at most 32 rows per sequence and kv head (single decoded tokens, a few drafted ones) last as long as
@@ -543,16 +552,14 @@ __device__ __forceinline__ int64_t row_slot(const PagedParams &p, int wave, int 
 //    4 g4 + i and 8 g4 + 4 + i for key 16 + 4 g4 + i; A = V^T for the same keys by two transposing reads;
 //    lane l accumulates dims 16 db + 4 g4 + i of row c16.
 template <int D, int NR, int NS>
-__global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
+__device__ __forceinline__ void row_runs(const PagedParams &p, int wave, __bf16 *ring) {
     constexpr int BN = 32, DC = D / 32, DB = D / 16, CPR = D / 8;
     constexpr int TILE = BN * D;  // elements of a step's K (or V)
     constexpr int LH = CPR / 4;   // 1 KB loads of 16 keys
     constexpr int LPS = 4 * LH;   // loads of a step
     static_assert(LH == 2 || LH % 4 == 0, "loads go out four at a time");
-    __shared__ __attribute__((aligned(16))) __bf16 ring[NS][2][TILE];
-
-    const int worker = over_kv_heads(p, blockIdx.x), kvh = blockIdx.x - worker * p.hkv;
-    const int lane = threadIdx.x, c16 = lane & 15, g4 = lane >> 4;
+    const int worker = over_kv_heads(p, wave), kvh = wave - worker * p.hkv;
+    const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
     RowLanes seqs = row_lanes(p, 0);
     int total = seqs.all;
     for (int base = 64; base < p.n_seq; base += 64) total += row_lanes(p, base).all;
@@ -573,7 +580,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
     const int vkey = 4 * g4 + (c16 >> 2), vdim = 4 * (c16 & 3);
     const int kbase = c16 * D + (g4 ^ unit_swz<CPR>(c16)) * 8;
     const int vbase = vkey * D + ((vdim >> 3) ^ unit_swz<CPR>(vkey)) * 8 + (vdim & 4);
-    const uint32_t ring_base = uniform((int)lds_addr(&ring[0][0][0]));
+    const uint32_t ring_base = uniform((int)lds_addr(ring));
     const char *k_head = reinterpret_cast<const char *>(p.k + kvh * p.k_sh);
     const char *v_head = reinterpret_cast<const char *>(p.v + kvh * p.v_sh);
     const uint64_t k_page = 2 * p.k_sp, v_page = 2 * p.v_sp;
@@ -686,7 +693,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
 #pragma unroll
             for (int s = 0; s < NS - 1; ++s) held[s] = held[s + 1];
             held[NS - 1] = page_ids(step + NS);
-            const __bf16 *kt = &ring[stage][0][0], *vt = &ring[stage][1][0];
+            const __bf16 *kt = ring + stage * (2 * TILE), *vt = kt + TILE;
             const int kt0 = key_first + 32 * step;
             const bool whole = mapped(ids.x) && mapped(ids.y) && block_full(kt0, khi, p0, p1, p.wl, p.wr);
             f32x4 sc[NR][2];
@@ -779,7 +786,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
                     *reinterpret_cast<bf16x4 *>(dst + 16 * db) = round4<false>(
                         o[r][db][0] * inv, o[r][db][1] * inv, o[r][db][2] * inv, o[r][db][3] * inv, bf16x4{});
             } else {
-                const int64_t slot = row_slot(p, blockIdx.x, slot_of) + row;
+                const int64_t slot = row_slot(p, wave, slot_of) + row;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
                     *reinterpret_cast<f32x4 *>(p.part_o + slot * D + 16 * db + 4 * g4) = o[r][db];
@@ -790,6 +797,30 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
             }
         }
     }
+}
+
+template <int D, int NR, int NS>
+__global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
+    __shared__ __attribute__((aligned(16))) __bf16 ring[NS * 2 * 32 * D];
+    row_runs<D, NR, NS>(p, blockIdx.x, ring);
+}
+
+// ----------------------------------------------------------------------------- both at once
+
+// A call of short and long sequences: the first `row_groups` workgroups, one per CU, run the short ones' rows with
+// as many waves as have their two stages in a tile's LDS, the others the long ones' tiles beside them, so that
+// what waits for memory and what waits for products share the CUs (one after the other, 40 decoding users
+// and two chunks of 2,048 rows at 32:8 heads of 128 took 844 us).
+template <int D>
+constexpr int kRowWaves = D == 64 ? 4 : D == 128 ? 2 : 1;
+
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void paged_both_kernel(PagedParams p, int row_groups) {
+    constexpr int kRing = 2 * 2 * 32 * D, kRows = kRowWaves<D> * kRing;
+    __shared__ __attribute__((aligned(16))) __bf16 ring[kRows > kTileLds<D> ? kRows : kTileLds<D>];
+    if ((int)blockIdx.x >= row_groups) return tile_item<D, SPLIT>(p, blockIdx.x - row_groups, ring);
+    const int wave = uniform(threadIdx.x >> 6), index = blockIdx.x * kRowWaves<D> + wave;
+    if (wave < kRowWaves<D> && index < p.workers * p.hkv) row_runs<D, 1, 2>(p, index, ring + wave * kRing);
 }
 
 // ----------------------------------------------------------------------------- the parts' sums

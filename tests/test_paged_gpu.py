@@ -78,6 +78,16 @@ def test_long_keys_are_split_over_workgroups(pe, heads, new):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("window", [(-1, -1), (700, -1)])
+def test_long_keys_of_short_and_long_sequences(pe, heads, window):
+    """Decoding users beside a chunk, the keys of both spread over workgroups; twice, with the same bits."""
+    new, keys = [1, 1, 70, 1, 2], [1500, 40, 1400, 931, 1025]
+    q, k, v, table, got = _check(pe, new, keys, heads, 48, window=window)
+    again = _run(pe, q, k, v, table, new, keys, window=window)
+    assert torch.equal(got, again)
+
+
 def test_a_bound_far_above_the_lengths_changes_nothing_but_rounding(pe):
     for slack in (0, 5000):
         _check(pe, [1, 2, 17], [300, 40, 17], (32, 8, 128), 16, slack=slack)
