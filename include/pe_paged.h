@@ -24,7 +24,8 @@
 extern "C" {
 #endif
 
-#define PE_PAGED_PAGE_MULTIPLE 16 /* page_size is a multiple of this */
+#define PE_PAGED_PAGE_MULTIPLE 16    /* page_size is a multiple of this */
+#define PE_PAGED_MAX_KEYS (1 << 29) /* largest max_seqlen_k and window, else PE_ATTN_EUNSUPPORTED */
 
 /* Attention of the new tokens (their k and v already in the pages):
  *     allowed(i, j) = j < seqlens_k && (window_left < 0 || i - j <= window_left)

@@ -47,8 +47,9 @@ PAGED_EXPORTED = (
     "pe_paged_append_fwd",
     "pe_copy_pages",
 )
-PAGE_MULTIPLE = 16      # PE_PAGED_PAGE_MULTIPLE
-ROTARY_MAX_PAIRS = 256  # PE_ROTARY_MAX_PAIRS
+PAGE_MULTIPLE = 16        # PE_PAGED_PAGE_MULTIPLE
+PAGED_MAX_KEYS = 1 << 29  # PE_PAGED_MAX_KEYS
+ROTARY_MAX_PAIRS = 256    # PE_ROTARY_MAX_PAIRS
 ROTARY_BF16, ROTARY_FP16, ROTARY_FP32 = 1, 2, 3
 
 

@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int64_t kCUs = 256;                      // compute units of an MI355X
-constexpr int32_t kMaxKeys = 1 << 30;              // key positions and what is added to them stay in 32 bits
+constexpr int32_t kMaxKeys = PE_PAGED_MAX_KEYS;  // key positions and what is added to them stay in 32 bits
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool row_stride(int64_t s) { return s >= 0 && (s & 7) == 0; }
@@ -144,10 +144,10 @@ PagedShape paged_shape(const pe_paged_args *a) {
     int64_t with = a->total_tokens * group / (s.few + 1);
     if (with > n) with = n;
     s.tiles = fill + with;
-    // Two workgroups per CU run at once. Calls of fewer tiles split their keys.
-    const int64_t at_once = 2 * kCUs;
+    // Two workgroups per CU run at once (head_dim 64: three). Calls of fewer tiles split their keys.
+    const int64_t at_once = (a->head_dim == 64 ? 3 : 2) * kCUs;
     if (fill * hkv < at_once && a->max_seqlen_k > 64 * pe::kChunkSteps) {
-        s.goal = (int32_t)(a->head_dim == 256 ? 3 * at_once / 2 : 2 * at_once);  // (its parts are the largest)
+        s.goal = (int32_t)((a->head_dim == 256 ? 3 : 4) * kCUs);  // (head_dim 256 has the largest parts)
         // The even share makes at most goal whole chunks, and one that is not of every tile; parts are left by
         // tiles of two chunks and more, so by at most 2 * goal.
         int64_t items = s.tiles + (s.goal + hkv - 1) / hkv;
@@ -259,8 +259,11 @@ int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedPar
 
 // ----------------------------------------------------------------------------- rotary positions
 
-// Tokens and heads of a workgroup: four tokens share a pass over the frequencies, but a call of few tokens
-// takes them one by one, and then spreads their heads, until it has two workgroups per CU.
+// Tokens and heads of a workgroup. Four tokens share a pass over the frequencies from two workgroups per CU
+// on (26,000 new tokens of 8:2 heads of 256 appended in 69 us, one by one in 89; rotary of 16,384 tokens of 8
+// heads of 128 12.1 against 15.0 us, of 40 heads 61 against 58). A call of fewer takes them one by one, and
+// below two workgroups per CU spreads their heads, four at least in each (64 tokens of 40 heads of 128 2.8 us,
+// whole tokens 3.2).
 void turn_shape(int64_t tokens, int heads, int *per, int *slice) {
     *per = tokens >= 4 * 2 * kCUs ? pe::kTurnTokens : 1;
     const int64_t groups = (tokens + *per - 1) / *per;

@@ -183,7 +183,7 @@ __device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes
     }
     sum = sum * p.hkv + p.goal - 1;
     const uint64_t steps = sum >> 32 ? sum / p.goal : (uint64_t)((uint32_t)sum / (uint32_t)p.goal);
-    return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 25)));
+    return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 23)));
 }
 
 struct TileItem {

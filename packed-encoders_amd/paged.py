@@ -135,7 +135,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     if native is not None and isinstance(k_pages, Tensor) and isinstance(page_table, Tensor):
         held = max_seqlen_k
         if held is None and k_pages.ndim == 4 and page_table.ndim == 2:
-            held = min(page_table.shape[1] * k_pages.shape[1], 1 << 30)
+            held = min(page_table.shape[1] * k_pages.shape[1], _lib.PAGED_MAX_KEYS)
         scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
         out = None if held is None else native.paged_attention(
             q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, max_seqlen, held, scale, window[0], window[1],
@@ -147,7 +147,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     if page_table.ndim != 2 or k_pages.ndim != 4:
         raise ValueError("page_table must be [n_seq, pages], k_pages [n_pages, page_size, heads, head_dim]")
     if max_seqlen_k is None:
-        max_seqlen_k = min(page_table.shape[1] * k_pages.shape[1], 1 << 30)
+        max_seqlen_k = min(page_table.shape[1] * k_pages.shape[1], _lib.PAGED_MAX_KEYS)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     options = (int(max_seqlen), int(max_seqlen_k), scale, int(window[0]), int(window[1]), bool(causal))
     return torch.ops.pe_hip.paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seqlens_k, *options)

@@ -50,7 +50,7 @@ def test_ctypes_structs_match_the_header_layout(pe, tmp_path, struct, cname):
     src = tmp_path / "layout.c"
     src.write_text('#include <stdio.h>\n#include "pe_paged.h"\nint main(void) {\n'
                    f'    printf("sizeof %zu 0\\n", sizeof({cname}));\n'
-                   '    printf("macros %d %d\\n", PE_PAGED_PAGE_MULTIPLE, PE_ROTARY_MAX_PAIRS);\n'
+                   '    printf("macros %d %d\\n", PE_PAGED_PAGE_MULTIPLE, PE_PAGED_MAX_KEYS - PE_ROTARY_MAX_PAIRS);\n'
                    f'{body}    return 0;\n}}\n')
     exe = tmp_path / "layout"
     subprocess.run([gcc, "-D__HIP_PLATFORM_AMD__", "-I", str(ROOT / "include"), "-I", hip_include, str(src), "-o",
@@ -60,7 +60,7 @@ def test_ctypes_structs_match_the_header_layout(pe, tmp_path, struct, cname):
         name, off, size = line.split()
         got[name] = (int(off), int(size))
     assert got.pop("sizeof")[0] == ctypes.sizeof(cls)
-    assert got.pop("macros") == (_lib.PAGE_MULTIPLE, _lib.ROTARY_MAX_PAIRS)
+    assert got.pop("macros") == (_lib.PAGE_MULTIPLE, _lib.PAGED_MAX_KEYS - _lib.ROTARY_MAX_PAIRS)
     assert got == {n: (getattr(cls, n).offset, getattr(cls, n).size) for n in names}
 
 
@@ -96,7 +96,7 @@ def _paged(**kw):
     ({"table_stride": -1}, -1), ({"q": None}, -1), ({"o": None}, -1), ({"k_pages": None}, -1), ({"v_pages": None}, -1),
     ({"page_table": None}, -1), ({"cu_seqlens": None}, -1), ({"seqlens_k": None}, -1), ({"q": (1 << 20) + 8}, -1),
     ({"k_stride_token": 1028}, -1), ({"k_stride_token": 64}, -1), ({"v_stride_page": -8}, -1), ({"o_stride_token": 4}, -1),
-    ({"max_seqlen_k": (1 << 30) + 1}, -2), ({"max_seqlen": 1 << 29}, -2), ({"k_stride_token": 1 << 26}, -2),
+    ({"max_seqlen_k": (1 << 29) + 1}, -2), ({"window_left": 1 << 30}, -2), ({"max_seqlen": 1 << 29}, -2), ({"k_stride_token": 1 << 26}, -2),
     ({"o_stride_token": 1 << 40}, -2), ({"o_stride_head": 1 << 40}, -2), ({"n_heads_q": 65544, "n_heads_kv": 8}, -2),
 ])
 def test_attention_arguments_are_rejected_before_any_launch(lib, kw, status):
@@ -118,7 +118,7 @@ def test_attention_needs_its_workspace(lib):
 
 def test_workspace_stays_bounded(lib):
     size = ctypes.c_size_t(0)
-    for n, tokens, longest, keys in [(1, 1, 1, 1 << 30), (1, 4096, 4096, 1 << 20), (300, 300, 1, 1 << 17), (8, 60000, 9000, 9000),
+    for n, tokens, longest, keys in [(1, 1, 1, 1 << 29), (1, 4096, 4096, 1 << 20), (300, 300, 1, 1 << 17), (8, 60000, 9000, 9000),
                                     (40, 700, 300, 30000), (2, 33, 32, 1 << 20)]:
         for hq, hkv, d in [(32, 8, 128), (8, 2, 256), (64, 64, 256), (12, 12, 64), (48, 1, 256), (640, 640, 256), (9000, 9000, 64)]:
             a = _paged(n_seq=n, total_tokens=tokens, max_seqlen=longest, max_seqlen_k=keys, n_heads_q=hq, n_heads_kv=hkv,

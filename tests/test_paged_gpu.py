@@ -432,6 +432,23 @@ def test_page_copy_refusals_copy_nothing(pe, src, dst):
     assert torch.equal(cache, before)
 
 
+def test_page_copies_in_a_graph(pe):
+    """The pairs are part of the captured launch; replays copy what the pages hold then."""
+    cache = torch.randn(3, 9, 16, 2, 64, device="cuda").bfloat16()
+    graph = torch.cuda.CUDAGraph()
+    pe.copy_pages(cache, [1, 2], [5, 6])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        pe.copy_pages(cache, [1, 1, 2], [5, 7, 6])
+    for _ in range(3):
+        cache.copy_(torch.randn_like(cache))
+        want = cache.clone()
+        want[:, [5, 7, 6]] = want[:, [1, 1, 2]]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache, want)
+
+
 def test_page_copy_refuses_other_shapes(pe):
     good = torch.zeros(9, 16, 1, 64, device="cuda")
     for bad in (good[0], good[..., ::2], good.expand(2, 9, 16, 1, 64)[:, :1].expand(2, 9, 16, 1, 64), [good, good[:8]],

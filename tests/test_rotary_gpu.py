@@ -71,6 +71,9 @@ def test_strides_and_leading_axes(pe):
     oracle.assert_within(pe.rotary(dev, shared.cuda(), inv.cuda()).reshape(120, 9, 64), want, bound)
     want, bound = oracle.rotate(rows[0], torch.full((30,), 7), inv)
     oracle.assert_within(pe.rotary(dev[0], torch.tensor(7).cuda(), inv.cuda()), want, bound)
+    one = dev[0, 3]  # [heads, head_dim], one position
+    want, bound = oracle.rotate(rows[0, 3:4], torch.tensor([41]), inv)
+    oracle.assert_within(pe.rotary(one, torch.tensor(41).cuda(), inv.cuda())[None], want, bound)
     # a broadcast row, and bases off 16 bytes
     one = dev[0, :1].expand(30, 9, 64)
     want, bound = oracle.rotate(rows[0, :1].expand(30, 9, 64), positions[0], inv)
