@@ -80,6 +80,7 @@ int check_paged(const pe_paged_args *a, bool need_pointers) {
 struct PagedShape {
     int32_t few;
     int row_blocks;   // of 16 rows
+    bool group;       // paged_group_kernel: a workgroup per sequence and kv head
     int32_t workers;  // waves per kv head
     int64_t tiles;    // items per kv head, at most
     int32_t goal;     // whole chunks its keys are split into, 0: not split
@@ -119,6 +120,26 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
     return (int32_t)best;
 }
 
+// Whether paged_group_kernel, a workgroup per sequence and kv head, ends sooner than waves with equal runs and a
+// second launch, by an estimate in microseconds for sequences of up to max_seqlen_k keys, half of that on
+// average. A group's waves take their share of the keys step by step (1 us each at head_dim 128, of four
+// waves, 0.7 at 64, 1.5 at 256, of two) after 5 us, in rounds of the workgroups that fit the chip, or at HBM's
+// rate; the runs take 11 us more than HBM does. Measured, runs against groups, n sequences of k keys each, 32:8
+// heads of 128: 1 x 64 5.9 / 5.2 us, 4 x 256 10.3 / 6.5, 1 x 1,024 10.5 / 12.2, 4 x 2,048 16 / 21, 32 x 256 18 /
+// 10, 64 x 512 37 / 31, 64 x 1,536 84 / 76, 256 x 64 27 / 38; 8:2 of 256: 4 x 256 11.2 / 10.2, 32 x 768 19 / 23,
+// 128 x 512 34 / 28; 12 of 64: 4 x 1,024 10.1 / 9.3, 128 x 512 51 / 41, 256 x 64 22 / 25. Past 2,048 keys the
+// longest sequence decides, and the runs are the even ones.
+bool pays_group(const pe_paged_args *a) {
+    const double keys = a->max_seqlen_k, units = (double)a->n_seq * a->n_heads_kv;
+    if (keys > 2048) return false;
+    const int d = a->head_dim;
+    const double step = d == 64 ? 0.7 : d == 128 ? 1.0 : 1.5, waves = d == 256 ? 2 : 4, at_once = (d == 64 ? 2 : 1) * kCUs;
+    const double rounds = (double)(int64_t)((units + at_once - 1) / at_once), steps = (double)(int64_t)((keys + 32 * waves - 1) / (32 * waves));
+    const double megabytes = 0.55 * units * keys * d * 4e-6;
+    const double by_steps = rounds * (5 + steps * step), by_bytes = 4.5 + megabytes / 5.7;
+    return (by_steps > by_bytes ? by_steps : by_bytes) < 11 + megabytes / 5.2;
+}
+
 PagedShape paged_shape(const pe_paged_args *a) {
     PagedShape s;
     std::memset(&s, 0, sizeof(s));
@@ -130,6 +151,8 @@ PagedShape paged_shape(const pe_paged_args *a) {
     if ((rows <= 32 || (uneven && group <= 16)) && steps < (int64_t)1 << 30) {
         s.few = rows > 16 && rows <= 32 ? 32 : 16;
         s.row_blocks = s.few / 16;
+        s.group = rows <= 32 && pays_group(a);
+        if (s.group) return s;
         const int waves = rows <= 32 ? row_waves(a->head_dim) : a->head_dim == 64 ? 4 : a->head_dim == 128 ? 2 : 1;
         int64_t workers = waves * kCUs / hkv;
         const int64_t most = (steps + pe::kRunSteps - 1) / pe::kRunSteps;
@@ -238,6 +261,12 @@ int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedPar
             hipLaunchKernelGGL((pe::paged_both_kernel<D, true>), grid, dim3(256), 0, stream, p, groups);
         else
             hipLaunchKernelGGL((pe::paged_both_kernel<D, false>), grid, dim3(256), 0, stream, p, groups);
+    } else if (s.group) {
+        const dim3 grid((unsigned)(a->n_seq * a->n_heads_kv)), threads(64 * pe::kGroupWaves<D>);
+        if (s.row_blocks == 1)
+            hipLaunchKernelGGL((pe::paged_group_kernel<D, 1>), grid, threads, 0, stream, p);
+        else
+            hipLaunchKernelGGL((pe::paged_group_kernel<D, 2>), grid, threads, 0, stream, p);
     } else if (s.row_blocks) {
         constexpr int NS = D == 128 ? 3 : 2;
         const dim3 grid((unsigned)(s.workers * a->n_heads_kv));

@@ -65,6 +65,12 @@ struct Lanes {
     int start, rows, lk;
 };
 
+// Whether the call serves a sequence: `rows` new tokens from packed row `start` on, lk keys.
+__device__ __forceinline__ bool served(const PagedParams &p, int start, int rows, int lk) {
+    return rows > 0 && rows <= p.max_seqlen && lk >= 0 && lk <= p.max_seqlen_k && lk <= (int64_t)p.max_pages * p.page &&
+           start >= 0 && (int64_t)start + rows <= p.total_q;
+}
+
 __device__ __forceinline__ Lanes lanes_from(const PagedParams &p, int base) {
     Lanes q;
     q.start = q.rows = q.lk = 0;
@@ -73,9 +79,7 @@ __device__ __forceinline__ Lanes lanes_from(const PagedParams &p, int base) {
         q.start = p.cu[s];
         const int L = p.cu[s + 1] - q.start;
         q.lk = p.lens[s];
-        if (L > 0 && L <= p.max_seqlen && q.lk >= 0 && q.lk <= p.max_seqlen_k && q.lk <= (int64_t)p.max_pages * p.page &&
-            q.start >= 0 && (int64_t)q.start + L <= p.total_q)
-            q.rows = L * p.group;
+        if (served(p, q.start, L, q.lk)) q.rows = L * p.group;
     }
     return q;
 }
@@ -555,22 +559,27 @@ __device__ __forceinline__ int64_t row_slot(const PagedParams &p, int wave, int 
 //  * O^T = V^T . P^T per 16 dims: B = the lane's own 8 probabilities, k-slot 8 g4 + i standing for key
 //    4 g4 + i and 8 g4 + 4 + i for key 16 + 4 g4 + i; A = V^T for the same keys by two transposing reads;
 //    lane l accumulates dims 16 db + 4 g4 + i of row c16.
+// The steps of one wave over a sequence's keys: what it adds up for each row.
+template <int D, int NR>
+struct RowSums {
+    f32x4 o[NR][D / 16];
+    float m[NR], l[NR];
+};
+
+struct RowWork {
+    int seq, start, nrows, lk, off, khi;  // the sequence: its rows, keys, key position of its first row
+    int key_first, steps;                 // the wave's part of its keys
+};
+
 template <int D, int NR, int NS>
-__device__ __forceinline__ void row_runs(const PagedParams &p, int wave, __bf16 *ring) {
+__device__ __forceinline__ void row_steps(const PagedParams &p, int kvh, const RowWork &w, __bf16 *ring, RowSums<D, NR> &sums) {
     constexpr int BN = 32, DC = D / 32, DB = D / 16, CPR = D / 8;
     constexpr int TILE = BN * D;  // elements of a step's K (or V)
     constexpr int LH = CPR / 4;   // 1 KB loads of 16 keys
     constexpr int LPS = 4 * LH;   // loads of a step
     static_assert(LH == 2 || LH % 4 == 0, "loads go out four at a time");
-    const int worker = over_kv_heads(p, wave), kvh = wave - worker * p.hkv;
     const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
-    RowLanes seqs = row_lanes(p, 0);
-    int total = seqs.all;
-    for (int base = 64; base < p.n_seq; base += 64) total += row_lanes(p, base).all;
-    const int run = row_run(p, total), first = worker * run;
-    if (first >= total) return;
-    const int last = min(total, first + run);
-
+    const int start = w.start, nrows = w.nrows, lk = w.lk, off = w.off, khi = w.khi, key_first = w.key_first, steps = w.steps;
     const int k_row = (int)p.k_st * 2, v_row = (int)p.v_st * 2;
     int koff[LH], voff[LH];
 #pragma unroll
@@ -590,6 +599,193 @@ __device__ __forceinline__ void row_runs(const PagedParams &p, int wave, __bf16 
     const uint64_t k_page = 2 * p.k_sp, v_page = 2 * p.v_sp;
     const float c2 = p.c;
 
+    const PageIds table = page_ids_of(p, w.seq);
+    // The ids of the pages that hold a step's two halves.
+    auto page_ids = [&](int step) {
+        const int key = key_first + 32 * step, top = p.max_pages - 1;
+        if (top < 0) return int2{-1, -1};
+        return int2{table[min(page_of(p, key), top)], table[min(page_of(p, key + 16), top)]};
+    };
+    auto mapped = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
+    auto issue = [&](int stage, int step, int2 ids) {
+        const uint32_t base = ring_base + stage * (4 * TILE);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int key0 = key_first + 32 * step + 16 * h, slot = key0 - page_of(p, key0) * p.page;
+            const int id = h ? ids.y : ids.x;
+            const int rows = mapped(id) ? min(p.page - slot, lk - key0) : 0;
+            const __amdgpu_buffer_rsrc_t k_rs = page_rows(k_head, mapped(id) ? id : 0, k_page, slot, k_row, rows, D);
+            const __amdgpu_buffer_rsrc_t v_rs = page_rows(v_head, mapped(id) ? id : 0, v_page, slot, v_row, rows, D);
+            const uint32_t kb = base + h * LH * 1024, vb = kb + 2 * TILE;
+            if constexpr (LH == 2) {
+                const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
+                const int o4[4] = {koff[0], koff[1], voff[0], voff[1]};
+                dma16x4(l4, o4, k_rs, v_rs);
+            } else {
+#pragma unroll
+                for (int j = 0; j < LH; j += 4) {
+                    const uint32_t l = kb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
+                    const int o4[4] = {koff[j], koff[j + 1], koff[j + 2], koff[j + 3]};
+                    dma16x4(l4, o4, k_rs, k_rs);
+                }
+#pragma unroll
+                for (int j = 0; j < LH; j += 4) {
+                    const uint32_t l = vb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
+                    const int o4[4] = {voff[j], voff[j + 1], voff[j + 2], voff[j + 3]};
+                    dma16x4(l4, o4, v_rs, v_rs);
+                }
+            }
+        }
+    };
+
+    // Query fragments: lane (c16, g4) holds dims 32 c + 8 g4 .. of row c16 of each block.
+    int pos[NR];
+    bf16x8 qf[NR][DC];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        const int row = 16 * r + c16, token = token_of(p, row), head = kvh * p.group + row - token * p.group;
+        pos[r] = off + token;
+        const __bf16 *src = p.q + (int64_t)(start + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g4;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) qf[r][c] = row < nrows ? ld_g16(src + 32 * c) : bf16x8{};
+    }
+    const int p0 = off, p1 = off + token_of(p, nrows - 1) + 1;  // key positions of the first row, past the last
+
+    auto &o = sums.o;
+    auto &m = sums.m;
+    auto &ls = sums.l;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[r][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[r] = kNegInf;
+        ls[r] = 0.0f;
+    }
+    int2 held[NS];  // page ids of the steps in the ring, and of the next to issue
+#pragma unroll
+    for (int s = 0; s < NS; ++s) held[s] = page_ids(s);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the sequence before has read its stages
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+        if (s < steps) issue(s, s, held[s]);
+    // The query rows' wait, here once: at their first use it would stand in the loop, and wait for the
+    // loads ahead in every step.
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[r][c]));
+    for (int step = 0; step < steps; ++step) {
+        // The stage of the step before is free once its reads are done; a step's loads are complete once at
+        // most the later steps' are in flight.
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        const int stage = step % NS, ahead = step + NS - 1;
+        if (ahead < steps) issue(ahead % NS, ahead, held[NS - 1]);
+        const int later = min(steps, ahead + 1) - step - 1;
+        if (NS >= 4 && later >= 3) wait_vmcnt<NS >= 4 ? 3 * LPS : 0>();
+        else if (NS >= 3 && later >= 2) wait_vmcnt<2 * LPS>();
+        else if (later >= 1) wait_vmcnt<LPS>();
+        else wait_vmcnt<0>();
+        const int2 ids = held[0];
+#pragma unroll
+        for (int s = 0; s < NS - 1; ++s) held[s] = held[s + 1];
+        held[NS - 1] = page_ids(step + NS);
+        const __bf16 *kt = ring + stage * (2 * TILE), *vt = kt + TILE;
+        const int kt0 = key_first + 32 * step;
+        const bool whole = mapped(ids.x) && mapped(ids.y) && block_full(kt0, khi, p0, p1, p.wl, p.wr);
+        f32x4 sc[NR][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) sc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                const bf16x8 ka = ld_s16(kt + 16 * b * D + (kbase ^ (32 * c)));
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    sc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[r][c], sc[r][b], 0, 0, 0);
+            }
+        }
+        bf16x8 pb[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if (!whole) {
+                uint32_t km = key_mask(kt0, g4, pos[r], khi, p.wl, p.wr);  // bit x: key kt0 + 4 g4 + x
+                const uint32_t low = (1u << (16 - 4 * g4)) - 1u;          // of the step's first 16 keys
+                km &= (mapped(ids.x) ? low : 0u) | (mapped(ids.y) ? ~low : 0u);
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[r][b][i] = mask_score(sc[r][b][i], km, 16 * b + i);
+            }
+            const f32x4 &a = sc[r][0], &z = sc[r][1];
+            const float mx =
+                fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+            // Raised only when a row exceeds it by 2^8; the four lanes of a row share m.
+            if (wave_any(mx * c2 > m[r] + 8.0f)) {
+                float top = fmaxf(mx, __shfl_xor(mx, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mnew = fmaxf(m[r], top * c2);
+                const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m[r] - mnew);
+                m[r] = mnew;
+                ls[r] *= alpha;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[r][db] *= alpha;
+            }
+            const float muse = m[r] == kNegInf ? 0.0f : m[r];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pb[r][i] = (__bf16)exp2_fast(fmaf(sc[r][i >> 2][i & 3], c2, -muse));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ls[r] = sum2(pb[r], i, ls[r]);
+        }
+        auto values = [&](int db) {
+            const __bf16 *at = vt + (vbase ^ (16 * db));
+            const bf16x4 lo = tr16(at), hi = tr16(at + 16 * D);
+            return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        uint32_t bad = 0;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            bf16x8 va = values(db);
+            if (!whole) bad |= clean8(va);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) o[r][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[r], o[r][db], 0, 0, 0);
+        }
+        if (wave_any(bad != 0)) {
+#pragma unroll 1
+            for (int key = 0; key < BN; ++key) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {  // dims 16 db + 4 g4 ..
+                    const int unit = (2 * db + (g4 >> 1)) ^ unit_swz<CPR>(key);
+                    const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vt + key * D + unit * 8 + 4 * (g4 & 1));
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const bool reach = reaches(p, pos[r], kt0 + key, khi);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[r][db][i] += reach ? only_nonfinite(v4[i]) : 0.0f;
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        ls[r] += __shfl_xor(ls[r], 16);
+        ls[r] += __shfl_xor(ls[r], 32);
+    }
+}
+
+template <int D, int NR, int NS>
+__device__ __forceinline__ void row_runs(const PagedParams &p, int wave, __bf16 *ring) {
+    constexpr int DB = D / 16;
+    const int worker = over_kv_heads(p, wave), kvh = wave - worker * p.hkv;
+    const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
+    RowLanes seqs = row_lanes(p, 0);
+    int total = seqs.all;
+    for (int base = 64; base < p.n_seq; base += 64) total += row_lanes(p, base).all;
+    const int run = row_run(p, total), first = worker * run;
+    if (first >= total) return;
+    const int last = min(total, first + run);
+
     int before = 0;  // steps of the sequences before seqs.base
     for (int x = first; x < last;) {
         while (before + seqs.all <= x) {
@@ -599,204 +795,42 @@ __device__ __forceinline__ void row_runs(const PagedParams &p, int wave, __bf16 
         const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + seqs.upto > x));
         const int begin = before + __builtin_amdgcn_readlane(seqs.upto - seqs.n, who);
         const int end = before + __builtin_amdgcn_readlane(seqs.upto, who);
-        const int start = __builtin_amdgcn_readlane(seqs.seq.start, who), nrows = __builtin_amdgcn_readlane(seqs.seq.rows, who);
-        const int lk = __builtin_amdgcn_readlane(seqs.seq.lk, who), off = lk - token_of(p, nrows);
-        int klo, khi;
-        keys_of(p, off, lk, 0, nrows, klo, khi);
-        const int key_first = klo + 32 * (x - begin), steps = min(last, end) - x;
+        RowWork w;
+        w.seq = seqs.base + who;
+        w.start = __builtin_amdgcn_readlane(seqs.seq.start, who);
+        w.nrows = __builtin_amdgcn_readlane(seqs.seq.rows, who);
+        w.lk = __builtin_amdgcn_readlane(seqs.seq.lk, who);
+        w.off = w.lk - token_of(p, w.nrows);
+        keys_of(p, w.off, w.lk, 0, w.nrows, w.key_first, w.khi);
+        w.key_first += 32 * (x - begin);
+        w.steps = min(last, end) - x;
         const bool whole_row = begin >= first && end <= last;  // no other wave has keys of these rows
         const int slot_of = begin < first ? 0 : 1;
-        x += steps;
-
-        const PageIds table = page_ids_of(p, seqs.base + who);
-        // The ids of the pages that hold a step's two halves.
-        auto page_ids = [&](int step) {
-            const int key = key_first + 32 * step, top = p.max_pages - 1;
-            if (top < 0) return int2{-1, -1};
-            return int2{table[min(page_of(p, key), top)], table[min(page_of(p, key + 16), top)]};
-        };
-        auto mapped = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
-        auto issue = [&](int stage, int step, int2 ids) {
-            const uint32_t base = ring_base + stage * (4 * TILE);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key0 = key_first + 32 * step + 16 * h, slot = key0 - page_of(p, key0) * p.page;
-                const int id = h ? ids.y : ids.x;
-                const int rows = mapped(id) ? min(p.page - slot, lk - key0) : 0;
-                const __amdgpu_buffer_rsrc_t k_rs = page_rows(k_head, mapped(id) ? id : 0, k_page, slot, k_row, rows, D);
-                const __amdgpu_buffer_rsrc_t v_rs = page_rows(v_head, mapped(id) ? id : 0, v_page, slot, v_row, rows, D);
-                const uint32_t kb = base + h * LH * 1024, vb = kb + 2 * TILE;
-                if constexpr (LH == 2) {
-                    const uint32_t l4[4] = {kb, kb + 1024, vb, vb + 1024};
-                    const int o4[4] = {koff[0], koff[1], voff[0], voff[1]};
-                    dma16x4(l4, o4, k_rs, v_rs);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < LH; j += 4) {
-                        const uint32_t l = kb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
-                        const int o4[4] = {koff[j], koff[j + 1], koff[j + 2], koff[j + 3]};
-                        dma16x4(l4, o4, k_rs, k_rs);
-                    }
-#pragma unroll
-                    for (int j = 0; j < LH; j += 4) {
-                        const uint32_t l = vb + j * 1024, l4[4] = {l, l + 1024, l + 2048, l + 3072};
-                        const int o4[4] = {voff[j], voff[j + 1], voff[j + 2], voff[j + 3]};
-                        dma16x4(l4, o4, v_rs, v_rs);
-                    }
-                }
-            }
-        };
-
-        // Query fragments: lane (c16, g4) holds dims 32 c + 8 g4 .. of row c16 of each block.
-        int pos[NR];
-        bf16x8 qf[NR][DC];
+        x += w.steps;
+        RowSums<D, NR> sums;
+        row_steps<D, NR, NS>(p, kvh, w, ring, sums);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int row = 16 * r + c16, token = token_of(p, row), head = kvh * p.group + row - token * p.group;
-            pos[r] = off + token;
-            const __bf16 *src = p.q + (int64_t)(start + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g4;
-#pragma unroll
-            for (int c = 0; c < DC; ++c) qf[r][c] = row < nrows ? ld_g16(src + 32 * c) : bf16x8{};
-        }
-        const int p0 = off, p1 = off + token_of(p, nrows - 1) + 1;  // key positions of the first row, past the last
-
-        f32x4 o[NR][DB];
-        float m[NR], ls[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-#pragma unroll
-            for (int db = 0; db < DB; ++db) o[r][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            m[r] = kNegInf;
-            ls[r] = 0.0f;
-        }
-        int2 held[NS];  // page ids of the steps in the ring, and of the next to issue
-#pragma unroll
-        for (int s = 0; s < NS; ++s) held[s] = page_ids(s);
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the sequence before has read its stages
-#pragma unroll
-        for (int s = 0; s < NS - 1; ++s)
-            if (s < steps) issue(s, s, held[s]);
-        // The query rows' wait, here once: at their first use it would stand in the loop, and wait for the
-        // loads ahead in every step.
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(qf[r][c]));
-        for (int step = 0; step < steps; ++step) {
-            // The stage of the step before is free once its reads are done; a step's loads are complete once at
-            // most the later steps' are in flight.
-            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-            const int stage = step % NS, ahead = step + NS - 1;
-            if (ahead < steps) issue(ahead % NS, ahead, held[NS - 1]);
-            const int later = min(steps, ahead + 1) - step - 1;
-            if (NS >= 4 && later >= 3) wait_vmcnt<NS >= 4 ? 3 * LPS : 0>();
-            else if (NS >= 3 && later >= 2) wait_vmcnt<2 * LPS>();
-            else if (later >= 1) wait_vmcnt<LPS>();
-            else wait_vmcnt<0>();
-            const int2 ids = held[0];
-#pragma unroll
-            for (int s = 0; s < NS - 1; ++s) held[s] = held[s + 1];
-            held[NS - 1] = page_ids(step + NS);
-            const __bf16 *kt = ring + stage * (2 * TILE), *vt = kt + TILE;
-            const int kt0 = key_first + 32 * step;
-            const bool whole = mapped(ids.x) && mapped(ids.y) && block_full(kt0, khi, p0, p1, p.wl, p.wr);
-            f32x4 sc[NR][2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) sc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < DC; ++c) {
-                    const bf16x8 ka = ld_s16(kt + 16 * b * D + (kbase ^ (32 * c)));
-#pragma unroll
-                    for (int r = 0; r < NR; ++r)
-                        sc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[r][c], sc[r][b], 0, 0, 0);
-                }
-            }
-            bf16x8 pb[NR];
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                if (!whole) {
-                    uint32_t km = key_mask(kt0, g4, pos[r], khi, p.wl, p.wr);  // bit x: key kt0 + 4 g4 + x
-                    const uint32_t low = (1u << (16 - 4 * g4)) - 1u;          // of the step's first 16 keys
-                    km &= (mapped(ids.x) ? low : 0u) | (mapped(ids.y) ? ~low : 0u);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[r][b][i] = mask_score(sc[r][b][i], km, 16 * b + i);
-                }
-                const f32x4 &a = sc[r][0], &z = sc[r][1];
-                const float mx =
-                    fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
-                // Raised only when a row exceeds it by 2^8; the four lanes of a row share m.
-                if (wave_any(mx * c2 > m[r] + 8.0f)) {
-                    float top = fmaxf(mx, __shfl_xor(mx, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const float mnew = fmaxf(m[r], top * c2);
-                    const float alpha = mnew == kNegInf ? 1.0f : exp2_fast(m[r] - mnew);
-                    m[r] = mnew;
-                    ls[r] *= alpha;
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) o[r][db] *= alpha;
-                }
-                const float muse = m[r] == kNegInf ? 0.0f : m[r];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) pb[r][i] = (__bf16)exp2_fast(fmaf(sc[r][i >> 2][i & 3], c2, -muse));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ls[r] = sum2(pb[r], i, ls[r]);
-            }
-            auto values = [&](int db) {
-                const __bf16 *at = vt + (vbase ^ (16 * db));
-                const bf16x4 lo = tr16(at), hi = tr16(at + 16 * D);
-                return bf16x8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-            uint32_t bad = 0;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                bf16x8 va = values(db);
-                if (!whole) bad |= clean8(va);
-#pragma unroll
-                for (int r = 0; r < NR; ++r) o[r][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[r], o[r][db], 0, 0, 0);
-            }
-            if (wave_any(bad != 0)) {
-#pragma unroll 1
-                for (int key = 0; key < BN; ++key) {
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {  // dims 16 db + 4 g4 ..
-                        const int unit = (2 * db + (g4 >> 1)) ^ unit_swz<CPR>(key);
-                        const bf16x4 v4 = *reinterpret_cast<const bf16x4 *>(vt + key * D + unit * 8 + 4 * (g4 & 1));
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            const bool reach = reaches(p, pos[r], kt0 + key, khi);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[r][db][i] += reach ? only_nonfinite(v4[i]) : 0.0f;
-                        }
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            float l = ls[r] + __shfl_xor(ls[r], 16);
-            l += __shfl_xor(l, 32);
             const int row = 16 * r + c16;
-            if (row >= nrows) continue;
+            if (row >= w.nrows) continue;
             if (whole_row) {
                 const int token = token_of(p, row), head = kvh * p.group + row - token * p.group;
-                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-                __bf16 *dst = p.o + (int64_t)(start + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g4;
+                const float l = sums.l[r], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+                __bf16 *dst = p.o + (int64_t)(w.start + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g4;
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
-                    *reinterpret_cast<bf16x4 *>(dst + 16 * db) = round4<false>(
-                        o[r][db][0] * inv, o[r][db][1] * inv, o[r][db][2] * inv, o[r][db][3] * inv, bf16x4{});
+                for (int db = 0; db < DB; ++db) {
+                    const f32x4 &o = sums.o[r][db];
+                    *reinterpret_cast<bf16x4 *>(dst + 16 * db) =
+                        round4<false>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, bf16x4{});
+                }
             } else {
                 const int64_t slot = row_slot(p, wave, slot_of) + row;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
-                    *reinterpret_cast<f32x4 *>(p.part_o + slot * D + 16 * db + 4 * g4) = o[r][db];
+                    *reinterpret_cast<f32x4 *>(p.part_o + slot * D + 16 * db + 4 * g4) = sums.o[r][db];
                 if (g4 == 0) {
-                    p.part_ml[2 * slot] = m[r];
-                    p.part_ml[2 * slot + 1] = l;
+                    p.part_ml[2 * slot] = sums.m[r];
+                    p.part_ml[2 * slot + 1] = sums.l[r];
                 }
             }
         }
@@ -807,6 +841,70 @@ template <int D, int NR, int NS>
 __global__ __launch_bounds__(64) void paged_row_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(16))) __bf16 ring[NS * 2 * 32 * D];
     row_runs<D, NR, NS>(p, blockIdx.x, ring);
+}
+
+// Small calls: a workgroup per sequence and kv head, its waves' sums added through LDS. No parts and no second
+// launch, at the price of one CU's rate for all of a sequence's keys.
+template <int D>
+constexpr int kGroupWaves = D == 256 ? 2 : 4;
+
+template <int D, int NR>
+__global__ __launch_bounds__(64 * kGroupWaves<D>) void paged_group_kernel(PagedParams p) {
+    constexpr int NW = kGroupWaves<D>, BM = 16 * NR, DB = D / 16, kRing = 2 * 2 * 32 * D;
+    __shared__ __attribute__((aligned(16))) __bf16 ring[NW * kRing];
+    __shared__ float stat[NW][2][BM];
+    static_assert(sizeof(ring) >= (size_t)NW * BM * D * 4, "the waves' sums fit the stages");
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
+    const int seq = over_kv_heads(p, blockIdx.x), kvh = blockIdx.x - seq * p.hkv;
+    RowWork w;
+    w.seq = seq;
+    w.start = p.cu[seq];
+    const int L = p.cu[seq + 1] - w.start;
+    w.lk = p.lens[seq];
+    if (!served(p, w.start, L, w.lk)) return;
+    w.nrows = L * p.group;
+    w.off = w.lk - L;
+    int klo;
+    keys_of(p, w.off, w.lk, 0, w.nrows, klo, w.khi);
+    const int steps = max(0, (w.khi - klo + 31) >> 5), per = (steps + NW - 1) / NW;
+    w.key_first = klo + 32 * per * wave;
+    w.steps = min(per, max(0, steps - per * wave));
+    RowSums<D, NR> sums;
+    row_steps<D, NR, 2>(p, kvh, w, ring + wave * kRing, sums);
+    __syncthreads();
+    float *all = reinterpret_cast<float *>(ring);  // [NW][BM][D]
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        const int row = 16 * r + c16;
+        if (g4 == 0) {
+            stat[wave][0][row] = sums.m[r];
+            stat[wave][1][row] = sums.l[r];
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+            *reinterpret_cast<f32x4 *>(all + (wave * BM + row) * D + 16 * db + 4 * g4) = sums.o[r][db];
+    }
+    __syncthreads();
+    for (int i = tid; i < w.nrows * (D / 4); i += 64 * NW) {
+        const int row = i / (D / 4), dim = 4 * (i - row * (D / 4));
+        float mx = stat[0][0][row];
+#pragma unroll
+        for (int j = 1; j < NW; ++j) mx = fmaxf(mx, stat[j][0][row]);
+        float l = 0.0f;
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+            const float weight = stat[j][0][row] == kNegInf ? 0.0f : exp2_fast(stat[j][0][row] - mx);
+            l = fmaf(stat[j][1][row], weight, l);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(all + (j * BM + row) * D + dim);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = fmaf(y[k], weight, x[k]);
+        }
+        const int token = token_of(p, row), head = kvh * p.group + row - token * p.group;
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        *reinterpret_cast<bf16x4 *>(p.o + (int64_t)(w.start + token) * p.o_st + (int64_t)head * p.o_sh + dim) =
+            round4<false>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv, bf16x4{});
+    }
 }
 
 // ----------------------------------------------------------------------------- both at once

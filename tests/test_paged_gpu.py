@@ -133,6 +133,13 @@ def test_masked_keys_may_hold_anything(pe, heads, junk):
     oracle.assert_within(got[40:], want[40:], bound[40:])
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("n,keys,new", [(1, 2047, 1), (3, 2049, 1), (40, 300, 1), (70, 65, 1), (2, 1500, 2), (9, 33, 4)])
+def test_equal_sequences(pe, heads, n, keys, new):
+    """Batches on both sides of the sizes that a workgroup per sequence and kv head serves."""
+    _check(pe, [new] * n, [keys] * n, heads, 48)
+
+
 @pytest.mark.parametrize("heads", [(32, 8, 128), (8, 2, 256), (12, 12, 64)])
 @pytest.mark.parametrize("new", [40, 4])
 def test_infinite_values_reach_the_rows_that_attend_to_them(pe, heads, new):
@@ -537,8 +544,9 @@ def test_calls_on_two_streams_at_once(pe):
         assert all(torch.equal(o, outs[0]) for o in outs)
 
 
-def test_decoding_steps_in_a_graph(pe):
-    """Append and attention captured once, then replayed step by step with the lengths and table updated in
+@pytest.mark.parametrize("width", [20, 200])
+def test_decoding_steps_in_a_graph(pe, width):
+    """Append and attention captured once, in one launch (tables of 320 keys) and in two with parts (3,200), then replayed step by step with the lengths and table updated in
     place and other work between the replays; each step as the eager calls give it."""
     hq, hkv, d, page = 8, 2, 128, 16
     cache = pe.PagedCache(1, 64, page, hkv, d)
@@ -549,13 +557,13 @@ def test_decoding_steps_in_a_graph(pe):
     kp, vp = cache.k[0], cache.v[0]
     kp.zero_()
     vp.zero_()
-    table, lens = torch.full((3, 20), -1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    table, lens = torch.full((3, width), -1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
     q = torch.zeros(3, hq, d, dtype=torch.bfloat16, device="cuda")
     k, v = (torch.zeros(3, hkv, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
 
     def step():
         turned = pe.paged_append(k, v, kp, vp, table, cu, lens, q=q, inv_freq=inv)
-        return pe.paged_attention(turned, kp, vp, table, cu, lens, 1)  # the table's 320 keys: a split call
+        return pe.paged_attention(turned, kp, vp, table, cu, lens, 1)
 
     with torch.inference_mode():
         side = torch.cuda.Stream()
@@ -570,7 +578,7 @@ def test_decoding_steps_in_a_graph(pe):
             if n == 13:
                 cache.truncate(seqs[2], 3)
             cache.extend(seqs, counts)
-            t, held = cache.batch(seqs, width=20)
+            t, held = cache.batch(seqs, width=width)
             table.copy_(t)
             lens.copy_(held)
             for x in (q, k, v):
