@@ -84,7 +84,7 @@ struct PagedShape {
     int32_t workers;  // waves per kv head
     int64_t tiles;    // items per kv head, at most
     int32_t goal;     // whole chunks its keys are split into, 0: not split
-    int32_t chunk;    // steps of a chunk, 0: from goal
+    int32_t chunk, least_chunk;  // steps of a chunk, 0: from goal, and then the least
     int64_t run_slots, tile_slots;  // rows of parts, at most
 };
 
@@ -95,10 +95,16 @@ struct PagedShape {
 // two stages 161 us, six of three 169 us, ten of two 182 us.
 int row_waves(int head_dim) { return head_dim == 64 ? 8 : head_dim == 128 ? 3 : 2; }
 
-// Steps of a chunk for a call of one sequence: its tiles, cut into c chunks each, run in rounds of `at_once`
-// workgroups (`most` items altogether), each as long as a chunk and what a workgroup costs beside (item, in steps of 64 keys), and the
-// parts are added (six steps' time per round). 512 new rows on 16,384 keys at 32:8 heads of 128, by rounds: 1
-// 154 us, 1.5 157, 2 163, 3 178; 700 rows 265, 208, 231, 222.
+// The least steps of 64 keys of a chunk: 4, or 8 where several sequences share the chip below head_dim 256
+// (eight chunks of U{20..200} rows on U{200..2000} keys at 32:8 heads of 128 47 against 40 us; 300 rows of 8:2 of
+// 256 on 900 keys 31 against 48).
+constexpr int64_t kChunkSteps = 4;
+
+// Steps of a chunk for a call of one sequence, 0: not split. Its tiles, cut into c chunks each, run in rounds of
+// `at_once` workgroups (`most` items altogether), each as long as a chunk and what a workgroup costs beside
+// (item, in steps of 64 keys); then the parts are added (four steps' time and six per round). 512 new rows
+// on 16,384 keys at 32:8 heads of 128, by rounds: 1 154 us, 1.5 157, 2 163, 3 178; 700 rows 265, 208, 231, 222;
+// 300 rows on 300 keys whole 11 us, with a second launch 16.
 int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t most) {
     const int64_t item = a->head_dim == 64 ? 6 : a->head_dim == 128 ? 3 : 2;
     const int wr = a->causal ? 0 : a->window_right;
@@ -108,10 +114,10 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
         if (band < reach) reach = band;
     }
     const int64_t steps = (reach + 63) / 64;
-    int64_t best = steps, least = (tiles + at_once - 1) / at_once * (steps + item);
-    for (int64_t c = 2; c * tiles <= most && c * pe::kChunkSteps <= steps; ++c) {
+    int64_t best = 0, least = (tiles + at_once - 1) / at_once * (steps + item);
+    for (int64_t c = 2; c * tiles <= most && c * kChunkSteps <= steps; ++c) {
         const int64_t chunk = (steps + c - 1) / c, items = c * tiles;
-        const int64_t cost = (items + at_once - 1) / at_once * (chunk + item) + 6 * items / at_once;
+        const int64_t cost = (items + at_once - 1) / at_once * (chunk + item) + 6 * items / at_once + 4;
         if (cost < least) {
             least = cost;
             best = chunk;
@@ -169,20 +175,24 @@ PagedShape paged_shape(const pe_paged_args *a) {
     s.tiles = fill + with;
     // Two workgroups per CU run at once (head_dim 64: three). Calls of fewer tiles split their keys.
     const int64_t at_once = (a->head_dim == 64 ? 3 : 2) * kCUs;
-    if (fill * hkv < at_once && a->max_seqlen_k > 64 * pe::kChunkSteps) {
-        s.goal = (int32_t)((a->head_dim == 256 ? 3 : 4) * kCUs);  // (head_dim 256 has the largest parts)
-        // The even share makes at most goal whole chunks, and one that is not of every tile; parts are left by
-        // tiles of two chunks and more, so by at most 2 * goal.
-        int64_t items = s.tiles + (s.goal + hkv - 1) / hkv;
-        int64_t longest = s.tiles * ((a->max_seqlen_k + 64 * pe::kChunkSteps - 1) / (64 * pe::kChunkSteps));
-        if (n == 1) {
-            const int64_t tiles = (rows + pe::kTileRows - 1) / pe::kTileRows;
-            s.chunk = chunk_of(a, tiles * hkv, at_once, 2 * s.goal);
-            items = longest = tiles * ((a->max_seqlen_k + 64 * s.chunk - 1) / (64 * (int64_t)s.chunk));
+    s.least_chunk = n > 1 && a->head_dim < 256 ? 8 : kChunkSteps;
+    if (fill * hkv >= at_once || a->max_seqlen_k <= 64 * s.least_chunk) return s;
+    s.goal = (int32_t)((a->head_dim == 256 ? 3 : 4) * kCUs);  // (head_dim 256 has the largest parts)
+    // The even share makes at most goal whole chunks, and one that is not of every tile; parts are left by
+    // tiles of two chunks and more, so by at most 2 * goal.
+    int64_t items = s.tiles + (s.goal + hkv - 1) / hkv;
+    int64_t longest = s.tiles * ((a->max_seqlen_k + 64 * s.least_chunk - 1) / (64 * s.least_chunk));
+    if (n == 1) {
+        const int64_t tiles = (rows + pe::kTileRows - 1) / pe::kTileRows;
+        s.chunk = chunk_of(a, tiles * hkv, at_once, 2 * s.goal);
+        if (s.chunk == 0) {
+            s.goal = 0;
+            return s;
         }
-        s.tiles = items < longest ? items : longest;
-        s.tile_slots = (longest * hkv < 2 * s.goal ? longest * hkv : 2 * s.goal) * pe::kTileRows;
+        items = longest = tiles * ((a->max_seqlen_k + 64 * s.chunk - 1) / (64 * (int64_t)s.chunk));
     }
+    s.tiles = items < longest ? items : longest;
+    s.tile_slots = (longest * hkv < 2 * s.goal ? longest * hkv : 2 * s.goal) * pe::kTileRows;
     return s;
 }
 
@@ -227,6 +237,7 @@ pe::PagedParams paged_params(const pe_paged_args *a, const PagedShape &s, void *
     p.workers = s.workers;
     p.goal = s.goal;
     p.chunk = s.chunk;
+    p.least_chunk = s.least_chunk;
     p.tile_slots = s.run_slots;
     p.total_q = a->total_tokens;
     p.c = a->softmax_scale * pe::kLog2e;

@@ -30,7 +30,7 @@ struct PagedParams {
     int32_t few;                    // sequences of at most this many rows are paged_row_kernel's (0: none)
     int32_t workers;                // its waves per kv head
     int32_t goal;                   // whole chunks that paged_tile_kernel's keys should come to, over the kv heads
-    int32_t chunk;                  // steps of a chunk, 0: from goal
+    int32_t chunk, least_chunk;     // steps of a chunk, 0: from goal, and then the least
     int32_t total_q;
     float c;                        // softmax_scale * log2(e)
     int64_t tile_slots;             // first slot of paged_tile_kernel's parts
@@ -148,7 +148,6 @@ __device__ __forceinline__ bool mapped16(const PagedParams &p, PageIds table, in
 // Items of paged_tile_kernel: a query tile of 128 rows over a chunk of its keys. Calls of few tiles split their
 // keys until they fill the chip, many tiles stay whole; sequences of any lengths are cut alike.
 constexpr int kTileRows = 128;
-constexpr int kChunkSteps = 4;  // of 64 keys, at least
 
 struct TileLanes {
     Lanes seq;
@@ -187,7 +186,7 @@ __device__ __forceinline__ int chunk_steps(const PagedParams &p, const TileLanes
     }
     sum = sum * p.hkv + p.goal - 1;
     const uint64_t steps = sum >> 32 ? sum / p.goal : (uint64_t)((uint32_t)sum / (uint32_t)p.goal);
-    return uniform(max(kChunkSteps, (int)min(steps, (uint64_t)1 << 23)));
+    return uniform(max(p.least_chunk, (int)min(steps, (uint64_t)1 << 23)));
 }
 
 struct TileItem {
