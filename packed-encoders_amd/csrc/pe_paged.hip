@@ -14,6 +14,7 @@
 namespace {
 
 constexpr int64_t kCUs = 256;                      // compute units of an MI355X
+constexpr int64_t kMaxGroups = 0xffffffff / 256;   // workgroups of 256 along a grid's axis: their threads count in 32 bits
 constexpr int32_t kMaxKeys = PE_PAGED_MAX_KEYS;  // key positions and what is added to them stay in 32 bits
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -64,16 +65,20 @@ int check_paged(const pe_paged_args *a, bool need_pointers) {
         if (!row_stride(s)) return PE_ATTN_EINVAL;
     if (a->k_stride_token < a->head_dim || a->v_stride_token < a->head_dim) return PE_ATTN_EINVAL;
     if (a->total_tokens > 1 && a->o_stride_token < a->head_dim) return PE_ATTN_EINVAL;
-    // A page's rows and a sequence's output rows are addressed by 32-bit offsets.
+    // A page's rows and a tile's output rows are addressed by 32-bit offsets.
     const int64_t limit = (int64_t)1 << 31;
     const int64_t page_span = a->k_stride_token > a->v_stride_token ? a->k_stride_token : a->v_stride_token;
     if (page_span >= limit / 2 / a->page_size) return PE_ATTN_EUNSUPPORTED;
     const int64_t head_span = a->n_heads_q > 1 ? (a->n_heads_q - 1) * (a->o_stride_head < limit ? a->o_stride_head : limit) : 0;
+    const int64_t tile_tokens = (pe::kTileRows - 1) / (a->n_heads_q / a->n_heads_kv) + 1;  // from its first token to its last
     if (a->o_stride_token >= limit || head_span >= limit ||
-        ((int64_t)(a->max_seqlen ? a->max_seqlen - 1 : 0) * a->o_stride_token + head_span + a->head_dim) * 2 >= limit)
+        (tile_tokens * a->o_stride_token + head_span + a->head_dim) * 2 >= limit)
         return PE_ATTN_EUNSUPPORTED;
     return PE_ATTN_OK;
 }
+
+// The new tokens of a sequence that the call serves, at most.
+int64_t longest_of(const pe_paged_args *a) { return a->max_seqlen < a->total_tokens ? a->max_seqlen : a->total_tokens; }
 
 // How a call runs: paged_row_kernel for sequences of at most `few` rows (times the heads of a kv head) when
 // row_blocks > 0, paged_tile_kernel for the others when tiles > 0.
@@ -149,15 +154,15 @@ bool pays_group(const pe_paged_args *a) {
 PagedShape paged_shape(const pe_paged_args *a) {
     PagedShape s;
     std::memset(&s, 0, sizeof(s));
-    const int64_t group = a->n_heads_q / a->n_heads_kv, rows = (int64_t)a->max_seqlen * group;
+    const int64_t group = a->n_heads_q / a->n_heads_kv, rows = longest_of(a) * group;
     const int64_t n = a->n_seq, hkv = a->n_heads_kv;
     // A sequence's steps of 32 keys (one at least), summed over the sequences in 32 bits.
     const int64_t steps = (a->max_seqlen_k > 32 ? ((int64_t)a->max_seqlen_k + 31) / 32 : 1) * n;
-    const bool uneven = n > 1 && 2 * (int64_t)a->total_tokens < n * a->max_seqlen;  // some sequences are short
+    const bool uneven = n > 1 && 2 * (int64_t)a->total_tokens < n * longest_of(a);  // some sequences are short
     if ((rows <= 32 || (uneven && group <= 16)) && steps < (int64_t)1 << 30) {
         s.few = rows > 16 && rows <= 32 ? 32 : 16;
         s.row_blocks = s.few / 16;
-        s.group = rows <= 32 && pays_group(a);
+        s.group = rows <= 32 && n * hkv <= kMaxGroups && pays_group(a);
         if (s.group) return s;
         const int waves = rows <= 32 ? row_waves(a->head_dim) : a->head_dim == 64 ? 4 : a->head_dim == 128 ? 2 : 1;
         int64_t workers = waves * kCUs / hkv;
@@ -264,7 +269,10 @@ int launch_merge(const pe_paged_args *a, const pe::PagedParams &p, hipStream_t s
 template <int D>
 int launch_paged(const pe_paged_args *a, const PagedShape &s, const pe::PagedParams &p, hipStream_t stream) {
     const int64_t blocks = s.tiles * a->n_heads_kv;
-    if (blocks > 0x7fffff00LL - 8 * kCUs || (int64_t)a->total_tokens * a->n_heads_q > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    // Every launch fits its grid: tiles and row waves in one, and the merge's waves, one per row and head at most.
+    const bool parts = s.run_slots || s.tile_slots;
+    if (blocks > kMaxGroups - 8 * kCUs || (parts && (int64_t)a->total_tokens * a->n_heads_q > 4 * kMaxGroups))
+        return PE_ATTN_EUNSUPPORTED;
     if (s.row_blocks && s.tiles) {
         const int groups = (int)((s.workers * a->n_heads_kv + pe::kRowWaves<D> - 1) / pe::kRowWaves<D>);
         const dim3 grid((unsigned)(blocks + groups));
@@ -316,12 +324,17 @@ template <typename T, int V>
 int launch_rotary(const pe_rotary_args *a, pe::RotaryParams &p, hipStream_t stream) {
     const int64_t groups = (a->n_tokens + p.per - 1) / p.per;
     if (groups > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
-    const dim3 grid((unsigned)groups, (unsigned)((a->n_heads + p.slice - 1) / p.slice));
-    if (a->interleaved)
-        hipLaunchKernelGGL((pe::rotary_kernel<T, V, true>), grid, dim3(256), 0, stream, p);
-    else
-        hipLaunchKernelGGL((pe::rotary_kernel<T, V, false>), grid, dim3(256), 0, stream, p);
-    return launched();
+    const int64_t heads = (a->n_heads + p.slice - 1) / p.slice;
+    for (p.group0 = 0; p.group0 < groups; p.group0 += kMaxGroups) {
+        const int64_t left = groups - p.group0;
+        const dim3 grid((unsigned)(left < kMaxGroups ? left : kMaxGroups), (unsigned)heads);
+        if (a->interleaved)
+            hipLaunchKernelGGL((pe::rotary_kernel<T, V, true>), grid, dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((pe::rotary_kernel<T, V, false>), grid, dim3(256), 0, stream, p);
+        if (const int status = launched()) return status;
+    }
+    return PE_ATTN_OK;
 }
 
 // Whether rows split into units of v elements: whole pieces of the turned and of the copied part.
@@ -450,6 +463,7 @@ int pe_paged_append_fwd(const pe_append_args *a, hipStream_t stream) {
     const int64_t heads = (int64_t)a->n_heads_q + 2 * (int64_t)a->n_heads_kv;
     if (heads > 65535 || pe::kTurnTokens * heads * a->head_dim > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
     turn_shape(a->total_tokens, (int)heads, &p.per, &p.slice);
+    if ((a->total_tokens + (int64_t)p.per - 1) / p.per > kMaxGroups) return PE_ATTN_EUNSUPPORTED;
     const dim3 grid((unsigned)((a->total_tokens + p.per - 1) / p.per), (unsigned)((heads + p.slice - 1) / p.slice));
     const bool pieces = in_pieces(8, a->head_dim, a->half, a->interleaved);
     if (pieces && a->interleaved)
@@ -489,7 +503,7 @@ int pe_copy_pages(void *const *bases, int32_t n_bases, int64_t page_stride, int6
     p.stride = page_stride;
     p.pieces = page_bytes / 16;
     const int64_t blocks = (p.pieces + 256 * pe::kCopyPieces - 1) / (256 * pe::kCopyPieces);
-    if (blocks > 0x7fffffffLL) return PE_ATTN_EUNSUPPORTED;
+    if (blocks > kMaxGroups) return PE_ATTN_EUNSUPPORTED;
     for (int32_t b = 0; b < n_bases; b += pe::kCopyBases) {
         const int32_t nb = n_bases - b < pe::kCopyBases ? n_bases - b : pe::kCopyBases;
         for (int32_t i = 0; i < nb; ++i) p.base[i] = static_cast<char *>(bases[b + i]);

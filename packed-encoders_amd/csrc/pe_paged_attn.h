@@ -498,10 +498,11 @@ __device__ __forceinline__ void tile_item(const PagedParams &p, int block, __bf1
         return;
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const __amdgpu_buffer_rsrc_t o_rs =
-        make_rsrc(p.o + (int64_t)t.start * p.o_st,
-                  (uint32_t)(((int64_t)(token_of(p, t.rows) - 1) * p.o_st + (p.hq - 1) * p.o_sh + D) * 2));
-    const int ooff = row < t.rows ? (int)((token * p.o_st + head * p.o_sh) * 2) : kVoidOffset;
+    // The output from the tile's first token on: a resource of its own tokens, whatever the sequence's length.
+    const int first = token_of(p, t.row0), last = token_of(p, min(t.rows, t.row0 + BM) - 1);
+    const __amdgpu_buffer_rsrc_t o_rs = make_rsrc(
+        p.o + (int64_t)(t.start + first) * p.o_st, (uint32_t)(((int64_t)(last - first) * p.o_st + (p.hq - 1) * p.o_sh + D) * 2));
+    const int ooff = row < t.rows ? (int)(((token - first) * p.o_st + head * p.o_sh) * 2) : kVoidOffset;
     store_block<DB, false>(o, inv, kg, o_rs, ooff, o_rs, 0);
 }
 

@@ -147,6 +147,7 @@ struct RotaryParams {
     const void *positions;
     const float *inv_freq;
     int64_t x_st, x_sh, tokens;
+    int64_t group0;  // the launch's first workgroup (a grid holds so many)
     int32_t heads, d, half, wide;  // wide: positions are int64, else int32
     int32_t per;                   // tokens of a workgroup
     int32_t slice;                 // heads of a workgroup (grid y)
@@ -156,7 +157,7 @@ struct RotaryParams {
 template <typename T, int V, bool PAIRS>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     __shared__ __attribute__((aligned(16))) float c[kTurnTokens * kTurnPairs], s[kTurnTokens * kTurnPairs];
-    const int64_t first = (int64_t)blockIdx.x * p.per;
+    const int64_t first = (p.group0 + blockIdx.x) * p.per;
     const int n = (int)min((int64_t)p.per, p.tokens - first);
     for (int i = threadIdx.x; i < n * p.half; i += 256) {
         const int t = i / p.half, pair = i - t * p.half;

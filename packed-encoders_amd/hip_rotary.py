@@ -45,6 +45,8 @@ def _check(x: Tensor, positions: Tensor, inv_freq: Tensor) -> None:
     lead = x.shape[:-2]
     if positions.ndim > len(lead) or any(p not in (1, n) for p, n in zip(positions.shape[::-1], lead[::-1])):
         raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {tuple(lead)}")
+    if max(x.shape[-2:]) >= 2**31:
+        raise ValueError("rotary's heads and head_dim fit 32 bits")
     _check_frequencies(inv_freq, x.shape[-1], x.device)
 
 
@@ -149,6 +151,10 @@ def rotary_frequencies(rot_dim: int, theta: float, *, scaling: str | None = None
         raise ValueError(f"unknown scaling {scaling!r}")
     if scaling in ("ramp", "bands") and (original is None or original < 1):
         raise ValueError(f"scaling {scaling!r} needs the original context length")
+    if scaling == "ramp" and not (theta > 1.0 and beta_fast >= beta_slow > 0.0):
+        raise ValueError("scaling 'ramp' needs a theta above 1 and beta_fast >= beta_slow > 0")
+    if scaling == "bands" and not high > low > 0.0:
+        raise ValueError("scaling 'bands' needs high > low > 0")
     if scaling == "ntk":
         if rot_dim < 4:
             raise ValueError("scaling 'ntk' needs a rot_dim of at least 4")

@@ -66,6 +66,12 @@ def _no_grad(what: str, *tensors: Tensor | None) -> None:
         raise ValueError(f"{what} is forward-only; call it under torch.no_grad()")
 
 
+def _fits(**values: int) -> None:
+    for name, x in values.items():
+        if not -2**31 <= x < 2**31:
+            raise ValueError(f"{name} {x} does not fit 32 bits")
+
+
 def _on_device(what: str, *tensors: Tensor | None) -> None:
     if any(t is not None and t.device.type == "cpu" for t in tensors):
         raise ValueError(f"{what} runs on the HIP device")
@@ -82,6 +88,8 @@ def _attention_impl(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
         raise ValueError("q must be bf16 [tokens, heads, head_dim] with the pages' head_dim")
     if k_pages.shape[2] < 1 or q.shape[1] < 1 or q.shape[1] % k_pages.shape[2]:
         raise ValueError("query heads must be a multiple of kv heads")
+    _fits(tokens=q.shape[0], heads=q.shape[1], max_seqlen=max_seqlen, max_seqlen_k=max_seqlen_k,
+          window_left=window_left, window_right=window_right)
     out = torch.empty(q.shape, dtype=_BF16, device=q.device)
     q = _rows(q)
     a = _lib.PagedArgs()
@@ -169,6 +177,7 @@ def _append_impl(q: Tensor | None, k: Tensor, v: Tensor, k_pages: Tensor, v_page
     if q is not None and (q.ndim != 3 or q.dtype != _BF16 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or
                           q.shape[1] < 1 or q.device != k.device):
         raise ValueError("q must be bf16 [tokens, heads, head_dim] beside k")
+    _fits(tokens=k.shape[0], heads=k.shape[1], head_dim=k.shape[2], query_heads=0 if q is None else q.shape[1])
     half = 0
     if inv_freq is not None:
         half = _check_frequencies(inv_freq, k.shape[2], k.device)
@@ -340,8 +349,9 @@ class PagedCache:
     def fork(self, seq: int) -> int:
         """A sequence of the same tokens, sharing their pages. The first of the two to extend a last page that
         is not full copies it."""
+        pages, length = list(self._pages[seq]), self._lengths[seq]
         child = self.open()
-        self._pages[child], self._lengths[child] = list(self._pages[seq]), self._lengths[seq]
+        self._pages[child], self._lengths[child] = pages, length
         for page in self._pages[child]:
             self._users[page] += 1
         return child

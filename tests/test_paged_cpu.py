@@ -290,6 +290,14 @@ def test_forks_share_pages_and_copy_a_last_page_once(pe, copies):
     assert cache.free_pages == 16
 
 
+def test_unknown_sequences_change_nothing(pe, copies):
+    cache = pe.PagedCache(1, 4, 16, 1, 64, device="cpu")
+    for call in (cache.fork, cache.close, lambda s: cache.extend([s], [1]), lambda s: cache.truncate(s, 0)):
+        with pytest.raises(KeyError):
+            call(0)
+    assert cache.free_pages == 4 and cache.open() == 0
+
+
 def test_a_full_last_page_is_not_copied(pe, copies):
     cache = _cache(pe)
     a = cache.open()
@@ -452,7 +460,11 @@ def test_ntk_frequencies_end_where_they_should(pe):
 
 @pytest.mark.parametrize("args,kw", [((7, 1e4), {}), ((0, 1e4), {}), ((64, 0.0), {}), ((64, 1e4), {"factor": 0.5}),
                                      ((64, 1e4), {"scaling": "cubic"}), ((64, 1e4), {"scaling": "ramp", "factor": 2.0}),
-                                     ((2, 1e4), {"scaling": "ntk", "factor": 2.0})])
+                                     ((2, 1e4), {"scaling": "ntk", "factor": 2.0}),
+                                     ((64, 1.0), {"scaling": "ramp", "original": 64}),
+                                     ((64, 1e4), {"scaling": "ramp", "original": 64, "beta_slow": 0.0}),
+                                     ((64, 1e4), {"scaling": "ramp", "original": 64, "beta_fast": 0.5}),
+                                     ((64, 1e4), {"scaling": "bands", "original": 64, "low": 4.0})])
 def test_frequency_refusals(pe, args, kw):
     with pytest.raises(ValueError):
         pe.rotary_frequencies(*args, **kw)

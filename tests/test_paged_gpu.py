@@ -305,6 +305,50 @@ def test_pages_past_two_gib(pe):
     assert torch.equal(big_k[n_pages - 40], big_k[n_pages - 1])
 
 
+def test_outputs_past_two_gib(pe):
+    """A sequence whose output passes 2 GiB: tiles address theirs from their first token."""
+    hq, hkv, d, page, n = 64, 1, 256, 64, 66000  # 32 KiB a token
+    gen = torch.Generator().manual_seed(21)
+    k, v, table = _cache([n], page, hkv, d, gen)
+    q = torch.randn(n, hq, d, device="cuda", dtype=torch.bfloat16)
+    cu, lens = oracle.bounds([n]).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    with torch.inference_mode():
+        got = pe.paged_attention(q, k.cuda(), v.cuda(), table.cuda(), cu, lens, n, window=(20, 0))
+    for at in (0, 32760, 65530, n - 6):  # the last but two either side of 1 and 2 GiB
+        rows = q[at:at + 6].cpu()
+        want, bound = oracle.attention(rows, k, v, table, [6], [at + 6], window=(20, 0))
+        oracle.assert_within(got[at:at + 6], want, bound, f"tokens from {at}")
+
+
+@pytest.mark.parametrize("new,keys", [([1], [300]), ([40], [1500]), ([1, 1, 3], [70, 0, 900]), ([100, 1], [100, 2000])])
+def test_loose_bounds(pe, new, keys):
+    """max_seqlen past the call's tokens and max_seqlen_k past its keys bound no less."""
+    hq, hkv, d, page = 8, 2, 128, 32
+    gen = torch.Generator().manual_seed(22)
+    k, v, table = _cache(keys, page, hkv, d, gen, columns=200)
+    q = torch.randn(sum(new), hq, d, generator=gen).bfloat16()
+    want, bound = oracle.attention(q, k, v, table, new, keys)
+    args = [x.cuda() for x in (q, k, v, table, oracle.bounds(new), torch.tensor(keys, dtype=torch.int32))]
+    with torch.inference_mode():
+        for longest in (max(new), 1000, 1 << 20):
+            for held in (max(keys), 6400, 1 << 20):
+                announce(f"new {new} keys {keys} bounds {longest} {held}")
+                got = pe.paged_attention(*args, longest, max_seqlen_k=held)
+                oracle.assert_within(got, want, bound, f"{longest} {held}")
+
+
+def test_bounds_that_32_bits_do_not_hold_are_refused(pe):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    pages = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    table, cu, lens = (torch.zeros(*s, dtype=torch.int32, device="cuda") for s in ((2, 1), (3,), (2,)))
+    args = (q, pages, pages.clone(), table, cu, lens)
+    with torch.inference_mode():
+        for longest, kw in [(1 << 32, {}), (1, dict(max_seqlen_k=(1 << 32) + 16)), (1, dict(window=((1 << 32) + 5, -1))),
+                            (1, dict(window=(-1, (1 << 33) - 1), causal=False))]:
+            with pytest.raises(ValueError):
+                pe.paged_attention(*args, longest, **kw)
+
+
 # ----------------------------------------------------------------------------- appends
 
 

@@ -48,6 +48,20 @@ def test_far_positions_keep_their_angles(pe, base):
         oracle.assert_within(got, *oracle.rotate(x, positions, inv), f"{base} {index}")
 
 
+def test_more_tokens_than_a_grid_holds(pe):
+    """A grid's axis has fewer than 2^32 threads, 256 for four tokens: the rest is another launch's."""
+    edge = (2 ** 32 - 1) // 256 * 4
+    n = edge + 700
+    x = torch.randn(n, 1, 2, device="cuda", dtype=torch.bfloat16)
+    positions = torch.arange(n, device="cuda", dtype=torch.int32)
+    inv = torch.ones(1)
+    got = pe.rotary(x, positions, inv.cuda())
+    for at in (0, edge - 300, n - 500):
+        part = slice(at, at + 500)
+        want = oracle.rotate(x[part].cpu(), positions[part].cpu(), inv)
+        oracle.assert_within(got[part], *want, f"tokens from {at}")
+
+
 def test_strides_and_leading_axes(pe):
     gen = torch.Generator().manual_seed(2)
     rows = torch.randn(4, 30, 9, 64, generator=gen).bfloat16()
