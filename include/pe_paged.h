@@ -12,7 +12,8 @@
  * An entry outside [0, n_pages) (-1 by convention) maps no page: attention treats its keys as masked,
  * pe_paged_append_fwd drops their rows.
  *
- * The call's new tokens are packed: sequence s has rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1, and
+ * The call's new tokens are packed: sequence s has rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1
+ * (cu_seqlens does not descend), and
  * they are the last of its seqlens_k[s] keys: row r of Lq sits at key position seqlens_k[s] - Lq + r.
  */
 #ifndef PE_PAGED_H
