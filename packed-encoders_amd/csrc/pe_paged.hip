@@ -131,6 +131,13 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
     return (int32_t)best;
 }
 
+// Keys that `tokens` neighbouring ones of a sequence reach, at most (from a multiple of 64 on).
+int64_t reach_of(const pe_paged_args *a, int64_t tokens) {
+    const int wr = a->causal ? 0 : a->window_right;
+    const int64_t band = a->window_left >= 0 && wr >= 0 ? (int64_t)a->window_left + wr + tokens + 63 : a->max_seqlen_k;
+    return band < a->max_seqlen_k ? band : a->max_seqlen_k;
+}
+
 // Whether paged_group_kernel, a workgroup per sequence and kv head, ends sooner than waves with equal runs and a
 // second launch, by an estimate in microseconds for sequences of up to max_seqlen_k keys, half of that on
 // average. A group's waves take their share of the keys step by step (1 us each at head_dim 128, of four
@@ -141,7 +148,7 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
 // 128 x 512 34 / 28; 12 of 64: 4 x 1,024 10.1 / 9.3, 128 x 512 51 / 41, 256 x 64 22 / 25. Past 2,048 keys the
 // longest sequence decides, and the runs are the even ones.
 bool pays_group(const pe_paged_args *a) {
-    const double keys = a->max_seqlen_k, units = (double)a->n_seq * a->n_heads_kv;
+    const double keys = (double)reach_of(a, longest_of(a)), units = (double)a->n_seq * a->n_heads_kv;
     if (keys > 2048) return false;
     const int d = a->head_dim;
     const double step = d == 64 ? 0.7 : d == 128 ? 1.0 : 1.5, waves = d == 256 ? 2 : 4, at_once = (d == 64 ? 2 : 1) * kCUs;

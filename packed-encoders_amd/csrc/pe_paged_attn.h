@@ -878,37 +878,56 @@ __global__ __launch_bounds__(64 * kGroupWaves<D>) void paged_group_kernel(PagedP
     w.steps = min(per, max(0, steps - per * wave));
     RowSums<D, NR> sums;
     row_steps<D, NR, 2>(p, kvh, w, ring + wave * kRing, sums);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+        if (g4 == 0) {
+            stat[wave][0][16 * r + c16] = sums.m[r];
+            stat[wave][1][16 * r + c16] = sums.l[r];
+        }
     __syncthreads();
+    // A row's largest maximum and the inverse of its sum, and the weight of sums at maximum m.
+    auto weight = [](float m, float mx) { return m == kNegInf ? 0.0f : exp2_fast(m - mx); };
+    auto normaliser = [&](int row, float &mx) {
+        mx = stat[0][0][row];
+#pragma unroll
+        for (int j = 1; j < NW; ++j) mx = fmaxf(mx, stat[j][0][row]);
+        float l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) l = fmaf(stat[j][1][row], weight(stat[j][0][row], mx), l);
+        return l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    };
+    // Where a thread adds more than two pieces, the waves weigh their own sums first (12 sequences of 8 drafted
+    // tokens at 8:2 heads of 256 15.0 against 16.8 us), else each piece is weighed where it is added (four of one
+    // token at 32:8 of 128 9.3 against 9.5).
+    constexpr bool kFirst = BM * (D / 4) > 2 * 64 * NW;
     float *all = reinterpret_cast<float *>(ring);  // [NW][BM][D]
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         const int row = 16 * r + c16;
-        if (g4 == 0) {
-            stat[wave][0][row] = sums.m[r];
-            stat[wave][1][row] = sums.l[r];
+        float mine = 1.0f;
+        if constexpr (kFirst) {
+            float mx;
+            mine = normaliser(row, mx);
+            mine *= weight(sums.m[r], mx);
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-            *reinterpret_cast<f32x4 *>(all + (wave * BM + row) * D + 16 * db + 4 * g4) = sums.o[r][db];
+            *reinterpret_cast<f32x4 *>(all + (wave * BM + row) * D + 16 * db + 4 * g4) = sums.o[r][db] * mine;
     }
     __syncthreads();
+#pragma unroll 4
     for (int i = tid; i < w.nrows * (D / 4); i += 64 * NW) {
         const int row = i / (D / 4), dim = 4 * (i - row * (D / 4));
-        float mx = stat[0][0][row];
-#pragma unroll
-        for (int j = 1; j < NW; ++j) mx = fmaxf(mx, stat[j][0][row]);
-        float l = 0.0f;
+        float mx, inv = 1.0f;
+        if constexpr (!kFirst) inv = normaliser(row, mx);
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
-            const float weight = stat[j][0][row] == kNegInf ? 0.0f : exp2_fast(stat[j][0][row] - mx);
-            l = fmaf(stat[j][1][row], weight, l);
             const f32x4 y = *reinterpret_cast<const f32x4 *>(all + (j * BM + row) * D + dim);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = fmaf(y[k], weight, x[k]);
+            if constexpr (kFirst) x += y;
+            else x += y * weight(stat[j][0][row], mx);
         }
         const int token = token_of(p, row), head = kvh * p.group + row - token * p.group;
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         *reinterpret_cast<bf16x4 *>(p.o + (int64_t)(w.start + token) * p.o_st + (int64_t)head * p.o_sh + dim) =
             round4<false>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv, bf16x4{});
     }
