@@ -100,6 +100,14 @@ struct PagedShape {
 // two stages 161 us, six of three 169 us, ten of two 182 us.
 int row_waves(int head_dim) { return head_dim == 64 ? 8 : head_dim == 128 ? 3 : 2; }
 
+// Keys that `tokens` neighbouring ones of a sequence reach, at most (from a multiple of 64 on).
+int64_t reach_of(const pe_paged_args *a, int64_t tokens) {
+    const int wr = a->causal ? 0 : a->window_right;
+    const int64_t band = a->window_left >= 0 && wr >= 0 ? (int64_t)a->window_left + wr + tokens + 63 : a->max_seqlen_k;
+    return band < a->max_seqlen_k ? band : a->max_seqlen_k;
+}
+int64_t tile_reach(const pe_paged_args *a) { return reach_of(a, (pe::kTileRows - 1) / (a->n_heads_q / a->n_heads_kv) + 3); }
+
 // The least steps of 64 keys of a chunk: 4, or 8 where several sequences share the chip below head_dim 256
 // (eight chunks of U{20..200} rows on U{200..2000} keys at 32:8 heads of 128 47 against 40 us; 300 rows of 8:2 of
 // 256 on 900 keys 31 against 48).
@@ -112,13 +120,7 @@ constexpr int64_t kChunkSteps = 4;
 // 300 rows on 300 keys whole 11 us, with a second launch 16.
 int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t most) {
     const int64_t item = a->head_dim == 64 ? 6 : a->head_dim == 128 ? 3 : 2;
-    const int wr = a->causal ? 0 : a->window_right;
-    int64_t reach = a->max_seqlen_k;
-    if (a->window_left >= 0 && wr >= 0) {
-        const int64_t band = (int64_t)a->window_left + wr + (pe::kTileRows - 1) / (a->n_heads_q / a->n_heads_kv) + 2 + 64;
-        if (band < reach) reach = band;
-    }
-    const int64_t steps = (reach + 63) / 64;
+    const int64_t steps = (tile_reach(a) + 63) / 64;
     int64_t best = 0, least = (tiles + at_once - 1) / at_once * (steps + item);
     for (int64_t c = 2; c * tiles <= most && c * kChunkSteps <= steps; ++c) {
         const int64_t chunk = (steps + c - 1) / c, items = c * tiles;
@@ -129,13 +131,6 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
         }
     }
     return (int32_t)best;
-}
-
-// Keys that `tokens` neighbouring ones of a sequence reach, at most (from a multiple of 64 on).
-int64_t reach_of(const pe_paged_args *a, int64_t tokens) {
-    const int wr = a->causal ? 0 : a->window_right;
-    const int64_t band = a->window_left >= 0 && wr >= 0 ? (int64_t)a->window_left + wr + tokens + 63 : a->max_seqlen_k;
-    return band < a->max_seqlen_k ? band : a->max_seqlen_k;
 }
 
 // Whether paged_group_kernel, a workgroup per sequence and kv head, ends sooner than waves with equal runs and a
@@ -156,6 +151,17 @@ bool pays_group(const pe_paged_args *a) {
     const double megabytes = 0.55 * units * keys * d * 4e-6;
     const double by_steps = rounds * (5 + steps * step), by_bytes = 4.5 + megabytes / 5.7;
     return (by_steps > by_bytes ? by_steps : by_bytes) < 11 + megabytes / 5.2;
+}
+
+// Whether the tiles of several sequences, `tiles` of the `at_once` that the chip holds, stay whole though
+// there are fewer: those of few steps (of 64 keys, for the longest that may come), the fewer the emptier the chip.
+// Measured at 32:8 heads of 128, split against whole, n chunks of r rows on k keys: 2 x 64 on 600 23 / 18 us, on
+// 1,000 24 / 24, on 2,000 26 / 42; 8 x 64 on 1,000 30 / 26, on 2,000 41 / 44; 8 x 200 on 1,000 67 / 38, on 4,000
+// 155 / 124, on U{400..2000} 48 / 43; 2 x 400 on 2,000 61 / 45, on U{400..2000} 30 / 40. 8:2 of 256: 8 x 200 on
+// 600 47 / 35, on 1,000 50 / 49, on 2,000 79 / 87; 2 x 64 on 600 25 / 31. 12 of 64: 8 x 200 on 1,000 27 / 21, on
+// 2,000 35 / 33; 24 x 40 on U{400..2000} 25 / 36.
+bool whole_tiles(const pe_paged_args *a, int64_t steps, int64_t tiles, int64_t at_once) {
+    return steps <= (a->head_dim == 256 ? 2 : 10) + (a->head_dim == 64 ? 48 : 64) * tiles / at_once;
 }
 
 PagedShape paged_shape(const pe_paged_args *a) {
@@ -188,7 +194,10 @@ PagedShape paged_shape(const pe_paged_args *a) {
     // Two workgroups per CU run at once (head_dim 64: three). Calls of fewer tiles split their keys.
     const int64_t at_once = (a->head_dim == 64 ? 3 : 2) * kCUs;
     s.least_chunk = n > 1 && a->head_dim < 256 ? 8 : kChunkSteps;
-    if (fill * hkv >= at_once || a->max_seqlen_k <= 64 * s.least_chunk) return s;
+    const int64_t reach_steps = (tile_reach(a) + 63) / 64;
+    if (fill * hkv >= at_once || reach_steps <= s.least_chunk) return s;
+    const int64_t likely = s.few ? fill : s.tiles, each = n * ((rows + pe::kTileRows - 1) / pe::kTileRows);
+    if (n > 1 && whole_tiles(a, reach_steps, (likely < each ? likely : each) * hkv, at_once)) return s;
     s.goal = (int32_t)((a->head_dim == 256 ? 3 : 4) * kCUs);  // (head_dim 256 has the largest parts)
     // The even share makes at most goal whole chunks, and one that is not of every tile; parts are left by
     // tiles of two chunks and more, so by at most 2 * goal.
