@@ -88,6 +88,21 @@ def test_long_keys_of_short_and_long_sequences(pe, heads, window):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("new", [1, 4, 8])
+@pytest.mark.parametrize("window,causal", [((86, -1), True), ((40, 30), False)])
+def test_windowed_tokens_on_long_keys(pe, heads, new, window, causal):
+    """Single and drafted tokens whose window is far shorter than their keys."""
+    _check(pe, [new, 1, new], [2500, 70, 4999], heads, 64, window=window, causal=causal)
+
+
+@pytest.mark.parametrize("heads", [(32, 8, 128), (8, 2, 256), (12, 12, 64)])
+def test_chunks_whole_and_split(pe, heads):
+    """Several chunks on keys few enough for whole tiles, and on more."""
+    for keys in ([130, 300], [900, 700], [2100, 400]):
+        _check(pe, [130, 40], keys, heads, 32)
+
+
 def test_a_bound_far_above_the_lengths_changes_nothing_but_rounding(pe):
     for slack in (0, 5000):
         _check(pe, [1, 2, 17], [300, 40, 17], (32, 8, 128), 16, slack=slack)
