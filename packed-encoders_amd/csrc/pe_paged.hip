@@ -134,14 +134,15 @@ int32_t chunk_of(const pe_paged_args *a, int64_t tiles, int64_t at_once, int64_t
 }
 
 // Whether paged_group_kernel, a workgroup per sequence and kv head, ends sooner than waves with equal runs and a
-// second launch, by an estimate in microseconds for sequences of up to max_seqlen_k keys, half of that on
-// average. A group's waves take their share of the keys step by step (1 us each at head_dim 128, of four
+// second launch, by an estimate in microseconds for sequences of up to max_seqlen_k keys in reach, half of that
+// on average. A group's waves take their share of the keys step by step (1 us each at head_dim 128, of four
 // waves, 0.7 at 64, 1.5 at 256, of two) after 5 us, in rounds of the workgroups that fit the chip, or at HBM's
 // rate; the runs take 11 us more than HBM does. Measured, runs against groups, n sequences of k keys each, 32:8
 // heads of 128: 1 x 64 5.9 / 5.2 us, 4 x 256 10.3 / 6.5, 1 x 1,024 10.5 / 12.2, 4 x 2,048 16 / 21, 32 x 256 18 /
 // 10, 64 x 512 37 / 31, 64 x 1,536 84 / 76, 256 x 64 27 / 38; 8:2 of 256: 4 x 256 11.2 / 10.2, 32 x 768 19 / 23,
 // 128 x 512 34 / 28; 12 of 64: 4 x 1,024 10.1 / 9.3, 128 x 512 51 / 41, 256 x 64 22 / 25. Past 2,048 keys the
-// longest sequence decides, and the runs are the even ones.
+// longest sequence decides, and the runs are the even ones. Under a window its reach counts (86 on 2,500 keys, one
+// token: 11.3 / 7.3, 8:2 of 256 12.6 / 10.5, 12 of 64 9.8 / 5.7).
 bool pays_group(const pe_paged_args *a) {
     const double keys = (double)reach_of(a, longest_of(a)), units = (double)a->n_seq * a->n_heads_kv;
     if (keys > 2048) return false;
